@@ -158,6 +158,45 @@ int mok_router_topk(const float* logits, int num_tokens, int num_experts, int to
 int mok_router_topk_bwd(const int32_t* top_experts_i32, const float* router_weights, const float* d_router_weights,
                         float* d_logits, int num_tokens, int num_experts, int topk, void* stream);
 
+/* Losses that keep a router's experts evenly used, with the counts behind them.  logits [num_tokens, num_experts] are f32 or
+ * (logits_bf16 != 0) bf16, num_experts <= 1024.  p = softmax(logits), or with `sigmoid` sigma(logits) over its row sum; per
+ * sequence s, f = E * counts / max(1, sum of counts), P = mean of p over the rows that count:
+ *   losses[0] = mean over the sequences with a row that counts of sum_e f_e P_e,  losses[1] = mean of logsumexp(logits)^2.
+ * A row counts if its token_mask byte is set (NULL: all) and it lies in a sequence: sequence_offsets int32
+ * [num_sequences + 1], not decreasing, sequence s = rows [offsets[s], offsets[s+1]) cut to [0, num_tokens) (NULL: one sequence
+ * of all rows, num_sequences = 1).  Rows that do not count are not read for the losses; a row whose logits are all -inf
+ * has p = 0 and adds nothing to losses[1].
+ * Either top_experts_in int64 [T, K] holds finished routes (ids outside [0, E) go nowhere, topk <= 255) and the next two are
+ * NULL, or it is NULL and the call also chooses the K largest logits of every row (topk <= 32; descending, lower expert
+ * first among equals) into top_experts_out int64 and router_weights f32 [T, K] (softmax, or sigmas over their sum, of those K).
+ * load: int32 [num_sequences, E] that stands for the counts in f (NULL: the counts).  Outputs: losses f32 [2], counts int32
+ * [num_sequences, E], coef f32 [num_sequences * E + 2] for mok_router_balance_bwd.  scratch: 16-byte aligned,
+ * mok_router_balance_scratch_bytes bytes, of this call alone until it has run.
+ * mok_router_balance_bwd writes all of d_logits (type of logits) from d_losses f32 [2] and, where the three are not NULL,
+ * from the gradient of the router weights (topk <= 32).
+ * No reference counterpart (the reference takes finished routes and returns no losses). */
+size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences);
+int mok_router_balance(const void* logits, int logits_bf16, int num_tokens, int num_experts, int topk, int num_sequences,
+                       int sigmoid, const int64_t* top_experts_in, int64_t* top_experts_out, float* router_weights,
+                       const uint8_t* token_mask, const int32_t* sequence_offsets, const int32_t* load, float* losses,
+                       int32_t* counts, float* coef, void* scratch, size_t scratch_bytes, void* stream);
+int mok_router_balance_bwd(const float* d_losses, const void* logits, int logits_bf16, const float* coef,
+                           const uint8_t* token_mask, const int32_t* sequence_offsets, const int64_t* top_experts,
+                           const float* router_weights, const float* d_router_weights, void* d_logits, int num_tokens,
+                           int num_experts, int topk, int num_sequences, int sigmoid, void* stream);
+
+/* counts int32 [num_sequences, num_experts] of routes [num_tokens, topk] (int64, or int32 with ids_i32 != 0; ids outside
+ * [0, num_experts) are not counted), of the rows that count as above.  No reference counterpart. */
+int mok_expert_counts(const void* top_experts, int ids_i32, int num_tokens, int topk, int num_experts, int num_sequences,
+                      const uint8_t* token_mask, const int32_t* sequence_offsets, int32_t* counts, void* stream);
+
+/* out = residual + dropout(x) over `count` elements, bf16 or f32 (residual NULL: dropout alone, which is also the gradient of
+ * x given that of out).  Element i is dropped if u_i < round(65536 p), else multiplied by 65536 / (65536 - round(65536 p)); u_i is
+ * 16-bit number (i & 7) of Philox4x32-10 with the counter (i >> 3 as 64 bits, 0, 0) and the key *seed (64 bits, read on
+ * the device).  The sum is rounded once.  out may be x or residual.  No reference counterpart. */
+int mok_dropout_add(const void* x, const void* residual, const int64_t* seed, void* out, int64_t count, int is_bf16, double p,
+                    void* stream);
+
 /* Single-rank epilogues that gather the routed rows through the schedule instead of reading a combine buffer:
  *   out[t] = bf16(y_shared[t] + sum_k w[t,k] * y_routed[row(t,k)])            (forward)
  *   d_x[t] = bf16(d_x_shared[t] + sum_k d_x_routed[row(t,k)]),

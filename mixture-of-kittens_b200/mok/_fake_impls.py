@@ -139,3 +139,41 @@ def _(logits, topk, all_gather_top_experts_buffer, rank):
 @_fake("mok::router_topk_bwd")
 def _(top_experts, router_weights, d_router_weights, num_experts):
     return _new(router_weights, (top_experts.shape[0], num_experts), torch.float32)
+
+
+def _balance_out(logits, sequence_offsets):
+    S, E = 1 if sequence_offsets is None else sequence_offsets.shape[0] - 1, logits.shape[1]
+    return _new(logits, (2,), torch.float32), _new(logits, (S, E), torch.int32), _new(logits, (S * E + 2,), torch.float32)
+
+
+@_fake("mok::router_balance")
+def _(logits, top_experts, token_mask=None, sequence_offsets=None, load=None, sigmoid=False):
+    return _balance_out(logits, sequence_offsets)
+
+
+@_fake("mok::router_topk_balance")
+def _(logits, topk, token_mask=None, sequence_offsets=None, sigmoid=False):
+    T = logits.shape[0]
+    return (_new(logits, (T, topk), torch.int64), _new(logits, (T, topk), torch.float32), *_balance_out(logits, sequence_offsets))
+
+
+@_fake("mok::router_balance_bwd")
+def _(d_losses, logits, coef, token_mask=None, sequence_offsets=None, top_experts=None, router_weights=None,
+      d_router_weights=None, sigmoid=False):
+    return torch.empty_like(logits)
+
+
+@_fake("mok::expert_counts")
+def _(top_experts, num_experts, token_mask=None, sequence_offsets=None):
+    S = 1 if sequence_offsets is None else sequence_offsets.shape[0] - 1
+    return _new(top_experts, (S, num_experts), torch.int32)
+
+
+@_fake("mok::dropout_add")
+def _(x, residual, seed, p):
+    return torch.empty_like(x)
+
+
+@_fake("mok::dropout_add_bwd")
+def _(d_out, seed, p):
+    return torch.empty_like(d_out)

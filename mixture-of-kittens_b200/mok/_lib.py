@@ -135,6 +135,13 @@ mok_fwd_epilogue = _sig("mok_fwd_epilogue", C.c_int, [vp, vp, vp, vp, C.c_int, C
 mok_bwd_epilogue = _sig("mok_bwd_epilogue", C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, vp])
 mok_router_topk = _sig("mok_router_topk", C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, vp, vp, u64p, C.c_int, C.c_int, vp])
 mok_router_topk_bwd = _sig("mok_router_topk_bwd", C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp])
+mok_router_balance_scratch_bytes = _sig("mok_router_balance_scratch_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int])
+mok_router_balance = _sig("mok_router_balance", C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp,
+                                                          vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp])
+mok_router_balance_bwd = _sig("mok_router_balance_bwd", C.c_int, [vp, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp, C.c_int, C.c_int,
+                                                                  C.c_int, C.c_int, C.c_int, vp])
+mok_expert_counts = _sig("mok_expert_counts", C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp])
+mok_dropout_add = _sig("mok_dropout_add", C.c_int, [vp, vp, vp, vp, C.c_int64, C.c_int, C.c_double, vp])
 mok_fwd_epilogue_rows = _sig("mok_fwd_epilogue_rows", C.c_int,
                              [vp, vp, vp, vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp])
 mok_bwd_epilogue_rows = _sig("mok_bwd_epilogue_rows", C.c_int,
@@ -188,6 +195,18 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is None or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _raw_stream(device.index)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def launch(device: torch.device, what: str, entry, *args) -> None:
+    """Calls `entry(*args, stream)` with `device` current, whatever device the caller has made current."""
+    if device.index is None or device.index == _current_device():
+        check(entry(*args, stream_ptr(device)), what)
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, stream_ptr(device)), what)
 
 
 def ptr_array(ptrs) -> C.Array:

@@ -367,6 +367,130 @@ def route_and_schedule(workspace: MoKWorkspace, config: MoKConfig, logits: torch
     return sched, top_experts, router_weights
 
 
+@dataclass(frozen=True, slots=True)
+class MoKBalance:
+    losses: torch.Tensor             # f32 [2]: balance loss, z-loss (differentiable)
+    counts: torch.Tensor             # int32 [num_sequences, num_experts]: routes of the tokens that count
+
+    @property
+    def balance(self) -> torch.Tensor:
+        return self.losses[0]
+
+    @property
+    def z(self) -> torch.Tensor:
+        return self.losses[1]
+
+
+def _sigmoid_score(score: str) -> bool:
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError("score must be 'softmax' or 'sigmoid'")
+    return score == "sigmoid"
+
+
+expert_counts = ops.expert_counts
+
+
+class _Balance(torch.autograd.Function):
+    """router_balance on the autograd tape without the dispatcher's cost (the operator's own formula does the same)."""
+
+    @staticmethod
+    def forward(ctx, logits, top_experts, token_mask, sequence_offsets, load, sigmoid):
+        out = ops.router_balance(logits, top_experts, token_mask, sequence_offsets, load, sigmoid)
+        ops._balance_setup(ctx, (logits, top_experts, token_mask, sequence_offsets, load, sigmoid), out)
+        return out
+
+    backward = staticmethod(torch.autograd.function.once_differentiable(ops._balance_backward))
+
+
+class _RouteBalanced(torch.autograd.Function):
+    """router_topk_balance on the autograd tape: one launch gives the gradient of the weights and of both losses."""
+
+    @staticmethod
+    def forward(ctx, logits, topk, token_mask, sequence_offsets, sigmoid):
+        out = ops.router_topk_balance(logits, topk, token_mask, sequence_offsets, sigmoid)
+        ops._topk_balance_setup(ctx, (logits, topk, token_mask, sequence_offsets, sigmoid), out)
+        return out
+
+    backward = staticmethod(torch.autograd.function.once_differentiable(ops._topk_balance_backward))
+
+
+def balance_loss(logits: torch.Tensor, top_experts: torch.Tensor, *, token_mask: torch.Tensor | None = None,
+                 sequence_offsets: torch.Tensor | None = None, score: str = "softmax",
+                 group: dist.ProcessGroup | None = None) -> MoKBalance:
+    """Balance loss, z-loss and per-expert counts of finished routes (int64 [T, K]) and the logits behind them (f32 or bf16
+    [T, E]); see `ops.router_balance`.  With `group` the loss uses the counts of all its ranks (one all-reduce of [1, E]
+    int32; averaged over the ranks the loss is then that of the global batch); `counts` stays local."""
+    sigmoid = _sigmoid_score(score)
+    load = None
+    if group is not None:
+        if sequence_offsets is not None:
+            raise ValueError("counts of a group belong to one loss over the whole batch: pass no sequence_offsets")
+        load = ops.expert_counts(top_experts, logits.shape[-1], token_mask)
+        dist.all_reduce(load, group=group)
+    losses, counts, _ = _Balance.apply(logits, top_experts, token_mask, sequence_offsets, load, sigmoid)
+    return MoKBalance(losses=losses, counts=counts)
+
+
+def route_balanced(logits: torch.Tensor, topk: int, *, token_mask: torch.Tensor | None = None,
+                   sequence_offsets: torch.Tensor | None = None, score: str = "softmax",
+                   group: dist.ProcessGroup | None = None) -> tuple[torch.Tensor, torch.Tensor, MoKBalance]:
+    """route() with the losses of `balance_loss` from the same pass over the logits: (top_experts int64 [T, K], router_weights
+    f32 [T, K], MoKBalance).  `score` "sigmoid" weighs the chosen experts by their sigmoids over the sum of them."""
+    sigmoid = _sigmoid_score(score)
+    experts, weights, losses, counts, _ = _RouteBalanced.apply(logits, topk, token_mask, sequence_offsets, sigmoid)
+    if group is not None:              # the loss needs the other ranks' counts, which follow from the choice
+        return experts, weights, balance_loss(logits, experts, token_mask=token_mask, sequence_offsets=sequence_offsets,
+                                              score=score, group=group)
+    return experts, weights, MoKBalance(losses=losses, counts=counts)
+
+
+def route_balanced_and_schedule(workspace: MoKWorkspace, config: MoKConfig, logits: torch.Tensor, *, num_local_experts: int,
+                                token_mask: torch.Tensor | None = None, sequence_offsets: torch.Tensor | None = None,
+                                score: str = "softmax", group: dist.ProcessGroup | None = None
+                                ) -> tuple[MoKSchedule, torch.Tensor, torch.Tensor, MoKBalance]:
+    """route_balanced() + build_schedule(): (schedule, top_experts, router_weights, MoKBalance)."""
+    if not isinstance(workspace, MoKWorkspace):
+        raise TypeError("workspace must be a MoKWorkspace")
+    if type(num_local_experts) is not int or num_local_experts <= 0:
+        raise ValueError("num_local_experts must be a positive integer")
+    if logits.ndim != 2 or logits.shape[0] != workspace.num_local_tokens:
+        raise ValueError("logits must have shape (num_local_tokens, num_experts)")
+    if logits.shape[1] != num_local_experts * workspace.ep_size:
+        raise ValueError("logits must have num_local_experts * ep_size columns")
+    experts, weights, balance = route_balanced(logits, workspace.topk, token_mask=token_mask, sequence_offsets=sequence_offsets,
+                                               score=score, group=group)
+    return build_schedule(workspace, config, experts, num_local_experts=num_local_experts), experts, weights, balance
+
+
+class _DropoutAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, seed, p):
+        out = ops.dropout_add(x, residual, seed, p)
+        ops._dropout_setup(ctx, (x, residual, seed, p), out)
+        return out
+
+    backward = staticmethod(torch.autograd.function.once_differentiable(ops._dropout_backward))
+
+
+def dropout_add(x: torch.Tensor, residual: torch.Tensor | None = None, *, p: float, training: bool = True,
+                seed: torch.Tensor | None = None) -> torch.Tensor:
+    """residual + dropout(x) (x alone without a residual), the layer's exit in a transformer block; see `ops.dropout_add`.
+    `seed` is an int64 tensor [1] on the device; without one it is drawn from torch's generator of that device, so
+    torch.manual_seed, activation checkpoints and captured graphs treat it like any other random number.  Not training, or
+    with p = 0, nothing is dropped and no seed drawn."""
+    if type(p) not in (float, int) or not 0 <= p <= 1:
+        raise ValueError("p must be a number in [0, 1]")
+    if not training or p == 0:
+        if residual is None:
+            return x
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError("residual must have the shape, dtype and device of x")
+        return x + residual
+    if seed is None:
+        seed = torch.randint(0, 2 ** 63 - 1, (1,), dtype=torch.int64, device=x.device)
+    return _DropoutAdd.apply(x, residual, seed, p)
+
+
 def validate_inputs(config: MoKConfig, workspace: MoKWorkspace, schedule: MoKSchedule, x: torch.Tensor,
                     router_weights: torch.Tensor, grad_output: torch.Tensor | None = None) -> None:
     if not isinstance(config, MoKConfig):

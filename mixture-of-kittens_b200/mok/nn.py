@@ -8,7 +8,8 @@ these wrappers sit directly on top of it and add nothing to the arithmetic:
   * ``MoKLayer``          — parameters of one expert-parallel rank (router, shared expert, local routed experts),
     ``forward(x)`` = router GEMM -> fused top-K router kernel -> schedule -> experts.  With ``mxfp8=True`` the
     routed bf16 master weights are quantised with ``ops.mxfp8_quantize`` whenever they changed, and their
-    gradients come back in bf16.
+    gradients come back in bf16.  ``forward(x, residual=r, return_balance=True)`` adds what a training step needs around
+    the experts: the router's balance and z-losses with the experts' counts, and residual + dropout at the exit.
 
 One workspace per (tokens, hidden, top-k) is shared by all layers of a model, as in the reference.
 """
@@ -69,12 +70,23 @@ class MoKLayer(torch.nn.Module):
 
     ``forward(x)`` routes with the layer's own router; ``forward(x, top_experts, router_weights)`` takes finished
     routes (int64 [T, K], f32 [T, K]) as ``functional.build_schedule`` / ``functional.forward`` do.
+
+    ``score`` "sigmoid" weighs the chosen experts by sigmoids instead of the softmax.  ``dropout`` is applied to the layer's
+    output while training; ``residual`` is added behind it in the same pass.  With ``return_balance`` the call returns
+    (output, functional.MoKBalance) for the tokens that ``token_mask`` and ``sequence_offsets`` leave (see
+    ``functional.balance_loss``); ``balance_group`` makes the loss that of the global batch of its ranks.
     """
 
     def __init__(self, hidden_size: int, intermediate_size: int, num_experts: int, topk: int, *,
                  group: dist.ProcessGroup | None = None, config: F.MoKConfig | None = None, mxfp8: bool = False,
-                 swiglu_limit: float | None = None, device: torch.device | str | None = None, seed: int | None = None):
+                 swiglu_limit: float | None = None, device: torch.device | str | None = None, seed: int | None = None,
+                 score: str = "softmax", dropout: float = 0.0, balance_group: dist.ProcessGroup | None = None):
         super().__init__()
+        if score not in ("softmax", "sigmoid"):
+            raise ValueError("score must be 'softmax' or 'sigmoid'")
+        if type(dropout) not in (float, int) or not 0 <= dropout <= 1:
+            raise ValueError("dropout must be a number in [0, 1]")
+        self.score, self.dropout, self.balance_group = score, dropout, balance_group
         self.group = group if group is not None else dist.group.WORLD
         ep_size = dist.get_world_size(self.group)
         if num_experts % ep_size != 0:
@@ -114,16 +126,30 @@ class MoKLayer(torch.nn.Module):
         return self._quantised
 
     def forward(self, x: torch.Tensor, top_experts: torch.Tensor | None = None,
-                router_weights: torch.Tensor | None = None) -> torch.Tensor:
+                router_weights: torch.Tensor | None = None, *, residual: torch.Tensor | None = None, return_balance: bool = False,
+                token_mask: torch.Tensor | None = None, sequence_offsets: torch.Tensor | None = None):
         if (top_experts is None) != (router_weights is None):
             raise ValueError("pass both top_experts and router_weights, or neither")
+        if return_balance and top_experts is not None:
+            raise ValueError("return_balance needs the layer's own router")
+        if not return_balance and (token_mask is not None or sequence_offsets is not None):
+            raise ValueError("token_mask and sequence_offsets say which tokens count for the losses: pass return_balance=True")
         ws = F.get_workspace(self.config, self.group, device=x.device, num_local_tokens=x.shape[0],
                              hidden_size=self.hidden_size, topk=self.topk)
+        balance = None
         if top_experts is None:
-            logits = torch.nn.functional.linear(x, self.router_weight.to(x.dtype)).float()
-            schedule, top_experts, router_weights = F.route_and_schedule(ws, self.config, logits,
-                                                                         num_local_experts=self.num_local_experts)
+            logits = torch.nn.functional.linear(x, self.router_weight.to(x.dtype))
+            if return_balance or self.score != "softmax":
+                schedule, top_experts, router_weights, balance = F.route_balanced_and_schedule(
+                    ws, self.config, logits, num_local_experts=self.num_local_experts, token_mask=token_mask,
+                    sequence_offsets=sequence_offsets, score=self.score, group=self.balance_group if return_balance else None)
+            else:
+                schedule, top_experts, router_weights = F.route_and_schedule(ws, self.config, logits.float(),
+                                                                             num_local_experts=self.num_local_experts)
         else:
             schedule = F.build_schedule(ws, self.config, top_experts, num_local_experts=self.num_local_experts)
-        return moe_experts(self.config, ws, schedule, x, router_weights, self.shared_gate, self.shared_up, self.shared_down,
-                           self.routed_gate, self.routed_up, self.routed_down, self.swiglu_limit, self.quantised())
+        out = moe_experts(self.config, ws, schedule, x, router_weights, self.shared_gate, self.shared_up, self.shared_down,
+                          self.routed_gate, self.routed_up, self.routed_down, self.swiglu_limit, self.quantised())
+        if residual is not None or (self.training and self.dropout):
+            out = F.dropout_add(out, residual, p=self.dropout, training=self.training)
+        return (out, balance) if return_balance else out

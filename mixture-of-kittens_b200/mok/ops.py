@@ -26,8 +26,8 @@ _EP_TEXT = "1, 2, 4, 8"
 # ------------------------------------------------------------------------------------------
 # operators whose body an eager call reaches directly
 # ------------------------------------------------------------------------------------------
-_EXACT = {"Tensor": (Tensor, torch.nn.Parameter), "int": (int,), "bool": (bool,), "list[int]": (list,),
-          "float | None": (float, int, type(None))}
+_EXACT = {"Tensor": (Tensor, torch.nn.Parameter), "Tensor | None": (Tensor, torch.nn.Parameter, type(None)), "int": (int,),
+          "bool": (bool,), "list[int]": (list,), "float": (float, int), "float | None": (float, int, type(None))}
 # keys under which a caller's kernel for plain CUDA or CPU tensors can be registered
 _KERNEL_KEYS = ("CUDA", "CPU", "AutogradCUDA", "AutogradCPU", "Autograd", "AutocastCUDA", "AutocastCPU", "ADInplaceOrView",
                 "BackendSelect", "CompositeExplicitAutograd", "CompositeExplicitAutogradNonFunctional", "CompositeImplicitAutograd")
@@ -108,7 +108,10 @@ def _operator(name: str, mutates_args, schema: str | None = None):
         op.mok_types = tuple(_EXACT[p.annotation] for p in params)
         op.mok_accepted = set()
         at = [i for i, exact in enumerate(op.mok_types) if exact[0] is Tensor]
-        op.mok_tensors = operator.itemgetter(*at) if len(at) > 1 else lambda args: (args[at[0]],)
+        if any(type(None) in exact and Tensor in exact for exact in op.mok_types):
+            op.mok_tensors = lambda args: [args[i] for i in at if i < len(args) and args[i] is not None]
+        else:
+            op.mok_tensors = operator.itemgetter(*at) if len(at) > 1 else lambda args: (args[at[0]],)
         op.mok_required = sum(p.default is inspect.Parameter.empty for p in params)
         op.mok_mutated = tuple(i for i, p in enumerate(params) if p.name in mutates_args)
         op.mok_other_kernels = frozenset("/".join(name.split("::") + [key]) for key in _KERNEL_KEYS) - torch.library._impls
@@ -923,3 +926,231 @@ def _router_backward(ctx, _d_experts, d_weights):
 
 
 torch.library.register_autograd("mok::router_topk", _router_backward, setup_context=_router_setup)
+
+
+# ------------------------------------------------------------------------------------------
+# losses that keep the experts evenly used, and the counts behind them (no reference op)
+# ------------------------------------------------------------------------------------------
+def _sequences(T: int, device, token_mask: Tensor | None, sequence_offsets: Tensor | None) -> int:
+    """Checks the two ways of saying which tokens count; returns the number of sequences."""
+    if token_mask is not None:
+        _need(token_mask.device == device and token_mask.dtype == torch.bool and token_mask.is_contiguous()
+              and tuple(token_mask.shape) == (T,), "token_mask must be a contiguous bool tensor [num_tokens] on the device of the logits "
+              "or routes")
+    if sequence_offsets is None:
+        return 1
+    _need(sequence_offsets.device == device and sequence_offsets.dtype == torch.int32 and sequence_offsets.is_contiguous()
+          and sequence_offsets.ndim == 1 and sequence_offsets.numel() >= 2,
+          "sequence_offsets must be a contiguous int32 tensor [num_sequences + 1] on the device of the logits or routes")
+    return sequence_offsets.numel() - 1
+
+
+def _balance_logits(logits: Tensor) -> tuple[int, int]:
+    _need(logits.is_cuda and logits.ndim == 2 and logits.is_contiguous(),
+          "logits must be a contiguous CUDA tensor of shape (num_tokens, num_experts)")
+    _need(logits.dtype in (torch.float32, torch.bfloat16), "logits must have dtype torch.float32 or torch.bfloat16", TypeError)
+    T, E = logits.shape
+    _need(0 < E <= 1024, "num_experts must be in [1, 1024]")
+    return T, E
+
+
+def _routes(top_experts: Tensor, dtypes=(torch.int64,)) -> tuple[int, int]:
+    _need(top_experts.is_cuda and top_experts.ndim == 2 and top_experts.is_contiguous(),
+          "top_experts must be a contiguous CUDA tensor of shape (num_tokens, topk)")
+    _need(top_experts.dtype in dtypes, f"top_experts must have dtype {' or '.join(map(str, dtypes))}", TypeError)
+    T, K = top_experts.shape
+    _need(0 < K <= 255, "topk must be in [1, 255]")
+    return T, K
+
+
+def _run_balance(logits: Tensor, K: int, top_in: Tensor | None, experts: Tensor | None, weights: Tensor | None,
+                 token_mask: Tensor | None, sequence_offsets: Tensor | None, load: Tensor | None, sigmoid: bool, what: str):
+    T, E = logits.shape
+    dev = logits.device
+    S = _sequences(T, dev, token_mask, sequence_offsets)
+    if load is not None:
+        _need(load.device == dev and load.dtype == torch.int32 and load.is_contiguous() and tuple(load.shape) == (S, E),
+              "load must be a contiguous int32 tensor (num_sequences, num_experts) on the device of the logits")
+    _need(type(sigmoid) is bool, "sigmoid must be a boolean", TypeError)
+    make = torch.empty if T > 0 else torch.zeros
+    losses = make(2, dtype=torch.float32, device=dev)
+    counts = make(S, E, dtype=torch.int32, device=dev)
+    coef = make(S * E + 2, dtype=torch.float32, device=dev)
+    if T > 0:
+        nbytes = _lib.mok_router_balance_scratch_bytes(T, E, S)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.launch(dev, what, _lib.mok_router_balance, logits.data_ptr(), logits.dtype == torch.bfloat16, T, E, K, S, sigmoid,
+                    _vp(top_in), _vp(experts), _vp(weights), _vp(token_mask), _vp(sequence_offsets), _vp(load), losses.data_ptr(),
+                    counts.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes)
+    return losses, counts, coef
+
+
+@_operator("mok::router_balance", mutates_args=())
+def router_balance(logits: Tensor, top_experts: Tensor, token_mask: Tensor | None = None, sequence_offsets: Tensor | None = None,
+                   load: Tensor | None = None, sigmoid: bool = False) -> tuple[Tensor, Tensor, Tensor]:
+    """(losses f32 [2] = (balance, z), counts int32 [num_sequences, num_experts], coef for `router_balance_bwd`) of finished routes.
+
+    With p = softmax(logits) (or sigmoid(logits) over its row sum), per sequence f_e = E c_e / sum c and P_e the mean of p_e
+    over the tokens that count: balance is sum_e f_e P_e, averaged over the sequences that hold a token that counts (1 when
+    everything is even); z is the mean of logsumexp(logits)^2.  A token counts if `token_mask` (bool [T]) is set and it lies in
+    [sequence_offsets[0], sequence_offsets[-1]) (int32, not decreasing; None: one sequence of all tokens).  Ids outside
+    [0, E) are routes that go nowhere.  `load` (int32, the shape of counts) stands for the local counts in f: counts that
+    ranks have added up.  Differentiable with respect to the logits."""
+    T, _ = _balance_logits(logits)
+    T_routes, K = _routes(top_experts)
+    _need(T_routes == T and top_experts.device == logits.device, "top_experts must have as many tokens as logits, on their device")
+    return _run_balance(logits, K, top_experts, None, None, token_mask, sequence_offsets, load, sigmoid, "router_balance")
+
+
+@_operator("mok::router_topk_balance", mutates_args=())
+def router_topk_balance(logits: Tensor, topk: int, token_mask: Tensor | None = None, sequence_offsets: Tensor | None = None,
+                        sigmoid: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """`router_topk` and `router_balance` in one pass over the logits: (top_experts int64 [T, K], router_weights f32 [T, K],
+    losses, counts, coef).  With `sigmoid` the weights are the chosen experts' sigmoids over their sum.  Every token is
+    routed, also those that do not count for the losses; a token without a logit above -inf gets weights of 0."""
+    T, E = _balance_logits(logits)
+    _need(type(topk) is int and 0 < topk <= min(32, E), "topk must be in [1, min(32, num_experts)]")
+    experts = torch.empty(T, topk, dtype=torch.int64, device=logits.device)
+    weights = torch.empty(T, topk, dtype=torch.float32, device=logits.device)
+    return (experts, weights, *_run_balance(logits, topk, None, experts, weights, token_mask, sequence_offsets, None, sigmoid,
+                                            "router_topk_balance"))
+
+
+@_operator("mok::router_balance_bwd", mutates_args=())
+def router_balance_bwd(d_losses: Tensor, logits: Tensor, coef: Tensor, token_mask: Tensor | None = None,
+                       sequence_offsets: Tensor | None = None, top_experts: Tensor | None = None, router_weights: Tensor | None = None,
+                       d_router_weights: Tensor | None = None, sigmoid: bool = False) -> Tensor:
+    """d_logits in the type of the logits, from the gradient of the losses (f32 [2]) and, where the three are given, from the
+    gradient of the router weights."""
+    T, E = _balance_logits(logits)
+    dev = logits.device
+    S = _sequences(T, dev, token_mask, sequence_offsets)
+    for name, t, n in (("d_losses", d_losses, 2), ("coef", coef, S * E + 2)):
+        _need(t.device == dev and tuple(t.shape) == (n,) and t.is_contiguous(), f"{name} must be contiguous [{n}] on the device of the logits")
+        _need(t.dtype == torch.float32, f"{name} must have dtype torch.float32", TypeError)
+    _need(type(sigmoid) is bool, "sigmoid must be a boolean", TypeError)
+    K = 1
+    given = [t is not None for t in (top_experts, router_weights, d_router_weights)]
+    _need(all(given) or not any(given), "top_experts, router_weights and d_router_weights come together or not at all")
+    if all(given):
+        T_routes, K = _routes(top_experts)
+        _need(T_routes == T and K <= 32 and top_experts.device == dev, "top_experts must be [num_tokens, topk <= 32] on the device of the logits")
+        for name, t in (("router_weights", router_weights), ("d_router_weights", d_router_weights)):
+            _need(t.device == dev and tuple(t.shape) == (T, K) and t.is_contiguous(), f"{name} must be contiguous and match top_experts")
+            _need(t.dtype == torch.float32, f"{name} must have dtype torch.float32", TypeError)
+    d_logits = torch.empty_like(logits)
+    if T > 0:
+        _lib.launch(dev, "router_balance_bwd", _lib.mok_router_balance_bwd, d_losses.data_ptr(), logits.data_ptr(),
+                    logits.dtype == torch.bfloat16, coef.data_ptr(), _vp(token_mask), _vp(sequence_offsets), _vp(top_experts),
+                    _vp(router_weights), _vp(d_router_weights), d_logits.data_ptr(), T, E, K, S, sigmoid)
+    return d_logits
+
+
+@_operator("mok::expert_counts", mutates_args=())
+def expert_counts(top_experts: Tensor, num_experts: int, token_mask: Tensor | None = None,
+                  sequence_offsets: Tensor | None = None) -> Tensor:
+    """Routes per expert, int32 [num_sequences, num_experts], of the tokens that count (see `router_balance`).  Ids int64 or
+    int32; those outside [0, num_experts) are not counted."""
+    T, K = _routes(top_experts, (torch.int64, torch.int32))
+    _need(type(num_experts) is int and 0 < num_experts <= 1024, "num_experts must be in [1, 1024]")
+    dev = top_experts.device
+    S = _sequences(T, dev, token_mask, sequence_offsets)
+    if T == 0:
+        return torch.zeros(S, num_experts, dtype=torch.int32, device=dev)
+    counts = torch.empty(S, num_experts, dtype=torch.int32, device=dev)
+    _lib.launch(dev, "expert_counts", _lib.mok_expert_counts, top_experts.data_ptr(), top_experts.dtype == torch.int32, T, K,
+                num_experts, S, _vp(token_mask), _vp(sequence_offsets), counts.data_ptr())
+    return counts
+
+
+def _balance_setup(ctx, inputs, output):
+    logits, _top, token_mask, sequence_offsets, _load, sigmoid = inputs
+    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.set_materialize_grads(False)
+    ctx.sigmoid = sigmoid
+    ctx.save_for_backward(logits, output[2], token_mask, sequence_offsets)
+
+
+def _balance_backward(ctx, d_losses, _d_counts, _d_coef):
+    logits, coef, token_mask, sequence_offsets = ctx.saved_tensors
+    d_logits = None if d_losses is None else router_balance_bwd(d_losses.contiguous(), logits, coef, token_mask, sequence_offsets,
+                                                                None, None, None, ctx.sigmoid)
+    return d_logits, None, None, None, None, None
+
+
+torch.library.register_autograd("mok::router_balance", _balance_backward, setup_context=_balance_setup)
+
+
+def _topk_balance_setup(ctx, inputs, output):
+    logits, _topk, token_mask, sequence_offsets, sigmoid = inputs
+    experts, weights, _losses, counts, coef = output
+    ctx.mark_non_differentiable(experts, counts, coef)
+    ctx.set_materialize_grads(False)
+    ctx.sigmoid = sigmoid
+    ctx.save_for_backward(logits, coef, token_mask, sequence_offsets, experts, weights)
+
+
+def _topk_balance_backward(ctx, _d_experts, d_weights, d_losses, _d_counts, _d_coef):
+    logits, coef, token_mask, sequence_offsets, experts, weights = ctx.saved_tensors
+    if d_weights is None and d_losses is None:
+        return None, None, None, None, None
+    d_losses = logits.new_zeros(2, dtype=torch.float32) if d_losses is None else d_losses.contiguous()
+    routes = (None, None, None) if d_weights is None else (experts, weights, d_weights.contiguous())
+    return (router_balance_bwd(d_losses, logits, coef, token_mask, sequence_offsets, *routes, ctx.sigmoid), None, None, None, None)
+
+
+torch.library.register_autograd("mok::router_topk_balance", _topk_balance_backward, setup_context=_topk_balance_setup)
+
+
+# ------------------------------------------------------------------------------------------
+# dropout from a counter-based generator at the layer's exit (no reference op)
+# ------------------------------------------------------------------------------------------
+def _dropout_args(x: Tensor, name: str, seed: Tensor, p: float) -> None:
+    _need(x.is_cuda and x.is_contiguous(), f"{name} must be a contiguous CUDA tensor")
+    _need(x.dtype in (torch.bfloat16, torch.float32), f"{name} must have dtype torch.bfloat16 or torch.float32", TypeError)
+    _need(seed.device == x.device and tuple(seed.shape) == (1,), f"seed must have shape (1,) on the device of {name}")
+    _need(seed.dtype == torch.int64, "seed must have dtype torch.int64", TypeError)
+    _need(type(p) in (float, int) and 0 <= p <= 1, "p must be a number in [0, 1]")
+
+
+def _run_dropout(x: Tensor, residual: Tensor | None, seed: Tensor, p: float, what: str) -> Tensor:
+    out = torch.empty_like(x)
+    if x.numel() > 0:
+        _lib.launch(x.device, what, _lib.mok_dropout_add, x.data_ptr(), _vp(residual), seed.data_ptr(), out.data_ptr(), x.numel(),
+                    x.dtype == torch.bfloat16, float(p))
+    return out
+
+
+@_operator("mok::dropout_add", mutates_args=())
+def dropout_add(x: Tensor, residual: Tensor | None, seed: Tensor, p: float) -> Tensor:
+    """residual + dropout(x): an element of x is dropped with probability p (rounded to a multiple of 2^-16) and otherwise
+    divided by 1 - p.  Which ones depends on `seed` (int64 [1], read on the device) and their flat index alone, so nothing is
+    stored for the backward pass.  Differentiable with respect to x and residual."""
+    _dropout_args(x, "x", seed, p)
+    if residual is not None:
+        _need(residual.device == x.device and residual.shape == x.shape and residual.is_contiguous(),
+              "residual must be contiguous and have the shape and device of x")
+        _need(residual.dtype == x.dtype, "residual must have the dtype of x", TypeError)
+    return _run_dropout(x, residual, seed, p, "dropout_add")
+
+
+@_operator("mok::dropout_add_bwd", mutates_args=())
+def dropout_add_bwd(d_out: Tensor, seed: Tensor, p: float) -> Tensor:
+    """Gradient of x in `dropout_add` (the residual's is d_out itself)."""
+    _dropout_args(d_out, "d_out", seed, p)
+    return _run_dropout(d_out, None, seed, p, "dropout_add_bwd")
+
+
+def _dropout_setup(ctx, inputs, output):
+    _x, residual, seed, p = inputs
+    ctx.p, ctx.with_residual = p, residual is not None
+    ctx.save_for_backward(seed)
+
+
+def _dropout_backward(ctx, d_out):
+    seed, = ctx.saved_tensors
+    d_x = dropout_add_bwd(d_out.contiguous(), seed, ctx.p) if ctx.needs_input_grad[0] else None
+    return d_x, d_out if ctx.with_residual else None, None, None
+
+
+torch.library.register_autograd("mok::dropout_add", _dropout_backward, setup_context=_dropout_setup)

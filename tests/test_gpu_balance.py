@@ -1,0 +1,404 @@
+"""GPU: balance and z-losses, per-expert counts and the router that gives them, against the 64-bit oracle.
+
+Tolerances, in units u = 2^-24 (half a step of f32):
+  * a softmax or sigmoid value: exp to 2 steps (4 u), its argument rounded to |difference| u, at most 40 u here, a sum of at
+    most 1024 positive terms in at most 32 + 5 additions (37 u), a reciprocal and a product (3 u): under 90 u; two such
+    factors, a dot product of the same length and the last products: 2 * 90 + 37 + 10 < 240 u of the terms' magnitude;
+  * the losses add at most 1024 rows a warp-lane in turn plus 8 warps and 592 / 8 + 8 slots and 1024 tiles of sequences here:
+    LOSS = 90 + 1200 u of the (positive) sum.  The z-loss squares lse, whose error is 90 u / sum + u |lse|: 3 * 90 u (|lse| + 1)^2;
+  * bf16 results: half a step more, 2^-8 of the value.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import training_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+GRAD, WEIGHT, LOSS = 240 * U, 180 * U, 1300 * U
+
+
+def make(dev, T, E, K, *, dtype=torch.float32, S=0, mask=False, seed=0, spread=2.0):
+    rng = np.random.default_rng(seed)
+    logits = torch.from_numpy((rng.standard_normal((T, E)) * spread + rng.standard_normal(E)).astype(np.float32)).to(dtype)
+    where = {}
+    if mask:
+        where["token_mask"] = torch.from_numpy(rng.random(T) < 0.8)
+    if S:
+        where["sequence_offsets"] = torch.from_numpy(np.sort(rng.integers(0, T + 1, S + 1)).astype(np.int32))
+    return logits, where
+
+
+def on(dev, where):
+    return {k: v.to(dev) for k, v in where.items()}
+
+
+def plain(where):
+    return {k: v.numpy() for k, v in where.items()}
+
+
+def check(dev, logits, K, where, sigmoid, *, experts=None, load=None, with_weights=True):
+    """Forward and backward of one call; `experts` given: finished routes."""
+    from mok import ops
+    T, E = logits.shape
+    rng = np.random.default_rng(7)
+    x = logits.to(dev)
+    score = dict(sigmoid=sigmoid)
+    chosen = O.select(logits.float().numpy(), K) if experts is None else experts
+    l64 = logits.double().requires_grad_(True)
+    ref = O.losses(l64, chosen, load=load, **plain(where), **score)
+    d_losses = torch.tensor([0.9, 0.02], dtype=torch.float32)
+    total = (ref * d_losses.double()).sum()
+    if experts is None:
+        got_e, got_w, got_l, got_c, coef = ops.router_topk_balance(x, K, sigmoid=sigmoid, **on(dev, where))
+        assert got_e.dtype == torch.int64 and np.array_equal(got_e.cpu().numpy(), chosen)
+        ref_w = O.weights(l64, chosen, sigmoid)
+        assert got_w.dtype == torch.float32 and (got_w.cpu().double() - ref_w).abs().max() <= WEIGHT
+        routes = ()
+        if with_weights:
+            d_w = torch.from_numpy(rng.standard_normal((T, K)).astype(np.float32))
+            total = total + (ref_w * d_w.double()).sum()
+            routes = (got_e, got_w, d_w.to(dev))
+    else:
+        ids = torch.from_numpy(experts).to(dev)
+        got_l, got_c, coef = ops.router_balance(x, ids, load=None if load is None else torch.from_numpy(load).to(dev),
+                                                sigmoid=sigmoid, **on(dev, where))
+        routes = ()
+    assert got_c.dtype == torch.int32 and np.array_equal(got_c.cpu().numpy(), O.expert_counts(chosen, E, **plain(where)))
+    rows = np.concatenate(O.counted_rows(T, **plain(where)))
+    lse = torch.logsumexp(l64.detach()[torch.from_numpy(rows)], 1)
+    lse = lse[lse != -np.inf]
+    ref_l = ref.detach()
+    got_l = got_l.cpu().double()
+    assert abs(float(got_l[0] - ref_l[0])) <= LOSS * float(ref_l[0]) + 1e-30
+    assert abs(float(got_l[1] - ref_l[1])) <= LOSS * float(ref_l[1]) + 270 * U * float(((lse.abs() + 1) ** 2).mean() if len(lse) else 0)
+    got = ops.router_balance_bwd(d_losses.to(dev), x, coef, None if "token_mask" not in where else where["token_mask"].to(dev),
+                                 None if "sequence_offsets" not in where else where["sequence_offsets"].to(dev),
+                                 *(routes or (None, None, None)), sigmoid)
+    assert got.dtype == logits.dtype
+    grad = torch.autograd.grad(total, l64)[0] if total.requires_grad else torch.zeros(T, E, dtype=torch.float64)
+    grad = torch.nan_to_num(grad, nan=0.0)              # rows without a finite logit: torch's 0 * (-inf - -inf)
+    # magnitude of the terms of each element
+    with torch.no_grad():
+        scale = torch.zeros(T, E, dtype=torch.float64)
+        counts = O.expert_counts(chosen, E, **plain(where)) if load is None else load
+        parts = O.counted_rows(T, **plain(where))
+        n, live = max(1, sum(map(len, parts))), max(1, sum(len(r) > 0 for r in parts))
+        for s, r in enumerate(parts):
+            if len(r):
+                a = torch.from_numpy(counts[s] * E / max(1, counts[s].sum()) / len(r) / live)
+                p, soft = O._scores(l64[r], sigmoid), torch.softmax(l64[r], 1)
+                scale[r] += 0.9 * p * (a + (p * a).sum(1, keepdim=True)) + 0.02 * 2 / n * torch.logsumexp(l64[r], 1).abs()[:, None] * soft
+                scale[r] += 0.02 * 2 / n * soft     # lse near 0 has an absolute error
+        if routes:
+            w, dw = ref_w, d_w.double().abs()
+            scale.scatter_add_(1, torch.from_numpy(chosen), w * (dw + (w * dw).sum(1, keepdim=True)))
+        scale = torch.nan_to_num(scale, nan=0.0)
+    bound = GRAD * scale + (grad.abs() * 2.0 ** -8 if logits.dtype == torch.bfloat16 else 0) + 1e-38
+    err = (got.cpu().double() - grad).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+    return got
+
+
+SHAPES = [(1, 1, 1), (1, 7, 3), (3, 8, 2), (17, 4, 4), (255, 16, 2), (513, 24, 5), (300, 33, 32), (1000, 64, 6), (777, 100, 7),
+          (2049, 128, 8), (640, 255, 8), (511, 256, 9), (300, 500, 6), (130, 512, 31), (200, 1000, 8), (97, 1024, 32)]
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,K", SHAPES)
+def test_routing_with_losses(cuda_device, T, E, K, dtype, sigmoid):
+    logits, where = make(cuda_device, T, E, K, dtype=dtype, seed=T + E)
+    check(cuda_device, logits, K, where, sigmoid)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("T,E,K,S,mask", [(513, 24, 5, 1, False), (2000, 64, 4, 37, True), (900, 16, 2, 300, True), (40, 8, 2, 90, False),
+                                          (5000, 256, 8, 3, False), (1111, 1000, 3, 5, True), (20000, 4, 1, 2, True)])
+def test_routing_on_packed_sequences(cuda_device, T, E, K, S, mask, sigmoid):
+    """Ragged and empty sequences, rows in front of, and behind them, masked rows."""
+    logits, where = make(cuda_device, T, E, K, S=S, mask=mask, seed=S)
+    check(cuda_device, logits, K, where, sigmoid)
+    check(cuda_device, logits, K, where, sigmoid, with_weights=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,K,S,mask", [(1, 1, 1, 0, False), (600, 33, 5, 0, True), (3000, 128, 200, 7, True), (444, 1024, 2, 11, False)])
+def test_losses_of_finished_routes(cuda_device, T, E, K, S, mask, dtype):
+    """Ids outside [0, E), the same expert twice, more than 32 routes, and counts that ranks have added up."""
+    logits, where = make(cuda_device, T, E, K, dtype=dtype, S=S, mask=mask, seed=K)
+    rng = np.random.default_rng(5)
+    experts = rng.integers(-2, E + 2, (T, K))
+    experts[:, -1] = experts[:, 0]
+    experts[0, 0] = 2 ** 40
+    check(cuda_device, logits, K, where, False, experts=experts)
+    load = rng.integers(0, 1000, (max(1, S), E)).astype(np.int32)
+    check(cuda_device, logits, K, where, True, experts=experts, load=load)
+
+
+def test_many_rows_and_few_experts(cuda_device):
+    logits, where = make(cuda_device, 70001, 8, 2, S=9, mask=True, seed=4)
+    check(cuda_device, logits, 2, where, False)
+
+
+def test_empty_rows_and_masked_experts(cuda_device):
+    """Experts switched off with -inf or the lowest value, rows without a finite logit, equal logits."""
+    logits, _ = make(cuda_device, 64, 20, 4, seed=1)
+    logits[:, 5:9] = -np.inf
+    logits[3] = -np.inf
+    logits[4, 1:] = -np.inf                                 # one logit left for four routes
+    logits[6] = 0.0                                         # ties: the lower expert first
+    logits[7, ::2] = 1.5
+    for sigmoid in (False, True):
+        got = check(cuda_device, logits, 4, {}, sigmoid)
+        assert bool((got[3] == 0).all()) and bool(torch.isfinite(got).all())
+    from mok import ops
+    low = torch.full((8, 6), torch.finfo(torch.float32).min, device=cuda_device)
+    low[:, 2] = 1.0
+    experts, weights, losses, _, coef = ops.router_topk_balance(low, 2)
+    assert experts.tolist() == [[2, 0]] * 8 and weights.tolist() == [[1.0, 0.0]] * 8 and torch.isfinite(losses).all()
+    assert torch.isfinite(ops.router_balance_bwd(torch.ones(2, device=cuda_device), low, coef)).all()
+
+
+def test_far_below_zero_sigmoids_do_not_vanish(cuda_device):
+    logits = torch.randn(200, 16, generator=torch.Generator().manual_seed(2)) * 3 - 150.0       # sigma underflows in f32
+    check(cuda_device, logits, 3, {}, True)
+    check(cuda_device, logits + 300.0, 3, {}, True)                                             # and saturates
+
+
+def test_masked_rows_may_hold_anything(cuda_device):
+    """NaN and infinities in rows that do not count reach neither the losses nor a gradient; in a row that counts they do."""
+    from mok import ops
+    logits, _ = make(cuda_device, 100, 12, 3, seed=9)
+    mask = torch.ones(100, dtype=torch.bool)
+    mask[10:20] = False
+    offsets = torch.tensor([0, 50, 90], dtype=torch.int32)
+    dirty = logits.clone()
+    dirty[10:15], dirty[15:20], dirty[92] = np.nan, np.inf, -np.inf
+    args = lambda l: (l.to(cuda_device), 3, mask.to(cuda_device), offsets.to(cuda_device))       # noqa: E731
+    clean_out, dirty_out = ops.router_topk_balance(*args(logits)), ops.router_topk_balance(*args(dirty))
+    assert torch.equal(clean_out[2], dirty_out[2]) and torch.equal(clean_out[3], dirty_out[3])
+    keep = mask.clone()
+    keep[92] = False
+    assert torch.equal(clean_out[0][keep], dirty_out[0][keep]) and torch.equal(clean_out[1][keep], dirty_out[1][keep])
+    d = torch.ones(2, device=cuda_device)
+    grads = [ops.router_balance_bwd(d, a[0], o[4], a[2], a[3]) for a, o in ((args(logits), clean_out), (args(dirty), dirty_out))]
+    assert torch.equal(*grads) and bool((grads[0][10:20] == 0).all()) and bool((grads[0][90:] == 0).all())
+    dirty[30, 2] = np.nan
+    assert bool(torch.isnan(ops.router_topk_balance(*args(dirty))[2]).all())
+    none = ops.router_topk_balance(logits.to(cuda_device), 3, torch.zeros(100, dtype=torch.bool, device=cuda_device))
+    assert none[2].tolist() == [0.0, 0.0] and int(none[3].sum()) == 0
+    assert int(ops.router_balance_bwd(d, logits.to(cuda_device), none[4], torch.zeros(100, dtype=torch.bool, device=cuda_device))
+               .count_nonzero()) == 0
+
+
+def test_routes_are_those_of_the_plain_router(cuda_device):
+    from mok import ops
+    for T, E, K in ((512, 128, 8), (300, 1000, 32), (64, 5, 5)):
+        logits = make(cuda_device, T, E, K, seed=E)[0].to(cuda_device)
+        experts, weights = ops.router_topk(logits, K)
+        got = ops.router_topk_balance(logits, K)
+        assert torch.equal(got[0], experts) and (got[1] - weights).abs().max() < 2e-6
+
+
+def test_logits_at_any_address(cuda_device):
+    """Rows that start on no 16-byte boundary: an odd number of experts, and a view one element into its storage."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for E in (64, 63, 65):
+            base = torch.randn(300 * E + 1, generator=torch.Generator().manual_seed(E)).to(dtype)
+            logits = base[1:].view(300, E)
+            from mok import ops
+            moved = base.to(cuda_device)[1:].view(300, E)
+            assert moved.data_ptr() % 16
+            a, b = ops.router_topk_balance(moved, 4), ops.router_topk_balance(logits.to(cuda_device).clone(), 4)
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+            d = torch.ones(2, device=cuda_device)
+            routes = (a[0], a[1], torch.ones_like(a[1]))
+            assert torch.equal(ops.router_balance_bwd(d, moved, a[4], None, None, *routes),
+                               ops.router_balance_bwd(d, logits.to(cuda_device).clone(), b[4], None, None, *routes))
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """More than 2^31 logits: the last rows are routed and get their gradient like any other."""
+    from mok import ops
+    T, E, K = (1 << 21) + 5, 1024, 2
+    logits = torch.zeros(T, E, dtype=torch.bfloat16, device=cuda_device)
+    tail = make(cuda_device, 50, E, K, dtype=torch.bfloat16, seed=8)[0]
+    logits[-50:] = tail.to(cuda_device)
+    offsets = torch.tensor([T - 50, T], dtype=torch.int32, device=cuda_device)
+    experts, weights, losses, counts, coef = ops.router_topk_balance(logits, K, None, offsets)
+    small = ops.router_topk_balance(tail.to(cuda_device), K)
+    assert torch.equal(experts[-50:], small[0]) and torch.equal(weights[-50:], small[1]) and torch.equal(counts, small[3])
+    assert experts[0].tolist() == [0, 1] and (losses - small[2]).abs().max() < 1e-4
+    d = torch.tensor([1.0, 0.1], device=cuda_device)
+    got = ops.router_balance_bwd(d, logits, coef, None, offsets)
+    assert int(got[:-50].count_nonzero()) == 0
+    want = ops.router_balance_bwd(d, tail.to(cuda_device), small[4])
+    assert (got[-50:].float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+@pytest.mark.parametrize("T,E,K,S,mask", [(1, 1, 1, 0, False), (513, 4, 2, 0, True), (7777, 256, 8, 40, True), (3000, 1024, 3, 700, False),
+                                          (100, 60, 255, 3, True)])
+def test_expert_counts(cuda_device, T, E, K, S, mask, dtype):
+    from mok import ops
+    _, where = make(cuda_device, T, 4, K, S=S, mask=mask, seed=T)
+    experts = np.random.default_rng(1).integers(-3, E + 3, (T, K))
+    got = ops.expert_counts(torch.from_numpy(experts).to(cuda_device, dtype), E, **on(cuda_device, where))
+    assert got.dtype == torch.int32 and np.array_equal(got.cpu().numpy(), O.expert_counts(experts, E, **plain(where)))
+
+
+def test_no_tokens(cuda_device):
+    from mok import functional as F, ops
+    logits = torch.zeros(0, 8, device=cuda_device)
+    offsets = torch.zeros(4, dtype=torch.int32, device=cuda_device)
+    experts, weights, losses, counts, coef = ops.router_topk_balance(logits, 2, None, offsets)
+    assert experts.shape == weights.shape == (0, 2) and losses.tolist() == [0, 0] and counts.tolist() == [[0] * 8] * 3
+    assert ops.router_balance_bwd(losses, logits, coef, None, offsets).shape == (0, 8)
+    assert F.expert_counts(experts, 8).tolist() == [[0] * 8]
+    assert F.balance_loss(logits, experts).losses.tolist() == [0, 0]
+
+
+def test_refusals(cuda_device):
+    from mok import ops
+    x = torch.zeros(8, 6, device=cuda_device)
+    ids = torch.zeros(8, 2, dtype=torch.int64, device=cuda_device)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=cuda_device)              # noqa: E731
+    mask = torch.ones(8, dtype=torch.bool, device=cuda_device)
+    for bad in (x.half(), x.double()):
+        with pytest.raises(TypeError):
+            ops.router_topk_balance(bad, 2)
+    with pytest.raises(TypeError):
+        ops.router_balance(x, ids.int())
+    with pytest.raises(TypeError):
+        ops.expert_counts(ids.short(), 6)
+    for call in (lambda: ops.router_topk_balance(x.t(), 2), lambda: ops.router_topk_balance(x, 0), lambda: ops.router_topk_balance(x, 7),
+                 lambda: ops.router_topk_balance(torch.zeros(2, 1025, device=cuda_device), 2), lambda: ops.router_topk_balance(x[0], 1),
+                 lambda: ops.router_topk_balance(torch.zeros(8, 64, device=cuda_device), 33),
+                 lambda: ops.router_topk_balance(x, 2, mask[:7]), lambda: ops.router_topk_balance(x, 2, mask.int()),
+                 lambda: ops.router_topk_balance(x, 2, mask.cpu()), lambda: ops.router_topk_balance(x, 2, None, i32(1)),
+                 lambda: ops.router_topk_balance(x, 2, None, i32(2).long()), lambda: ops.router_topk_balance(x, 2, None, i32(2, 2)),
+                 lambda: ops.router_balance(x, ids[:7]), lambda: ops.router_balance(x, ids.t()), lambda: ops.router_balance(x, ids.cpu()),
+                 lambda: ops.router_balance(x, ids, None, None, i32(6)), lambda: ops.router_balance(x, ids, None, i32(4), i32(1, 6)),
+                 lambda: ops.expert_counts(ids, 0), lambda: ops.expert_counts(ids, 1025), lambda: ops.expert_counts(ids[0], 6)):
+        with pytest.raises(ValueError):
+            call()
+    g, coef = torch.ones(2, device=cuda_device), torch.ones(8, device=cuda_device)
+    w = torch.ones(8, 2, device=cuda_device)
+    for args in ((g[:1], x, coef), (g, x, coef[:7]), (g, x, coef, None, i32(3)), (g, x, coef, None, None, ids, w),
+                 (g, x, coef, None, None, ids, w, w[:, :1]), (g, x, coef, None, None, ids[:4], w, w), (g.cpu(), x, coef)):
+        with pytest.raises(ValueError):
+            ops.router_balance_bwd(*args)
+    with pytest.raises(TypeError):
+        ops.router_balance_bwd(g.double(), x, coef)
+
+
+def test_gradients_through_the_functional_calls(cuda_device):
+    """The autograd functions and the operators' own formulas give the bytes of the explicit calls; unused outputs cost nothing."""
+    from mok import functional as F, ops
+    logits, where = make(cuda_device, 600, 40, 4, S=5, mask=True, seed=12)
+    where = on(cuda_device, where)
+    mask, off = where["token_mask"], where["sequence_offsets"]
+    x = logits.to(cuda_device).requires_grad_(True)
+    d_w = torch.randn(600, 4, device=cuda_device)
+    d_l = torch.tensor([0.3, 0.01], device=cuda_device)
+    for score in ("softmax", "sigmoid"):
+        experts, weights, bal = F.route_balanced(x, 4, score=score, **where)
+        e, w, losses, counts, coef = ops.router_topk_balance(x.detach(), 4, mask, off, score == "sigmoid")
+        assert torch.equal(experts, e) and torch.equal(weights, w) and torch.equal(bal.losses, losses) and torch.equal(bal.counts, counts)
+        want = ops.router_balance_bwd(d_l, x.detach(), coef, mask, off, e, w, d_w, score == "sigmoid")
+        got, = torch.autograd.grad([weights, bal.losses], x, [d_w, d_l])
+        assert torch.equal(got, want)
+        through_op = ops.router_topk_balance(x, 4, mask, off, score == "sigmoid")
+        got, = torch.autograd.grad([through_op[1], through_op[2]], x, [d_w, d_l])
+        assert torch.equal(got, want)
+        experts, weights, bal = F.route_balanced(x, 4, score=score, **where)
+        got, = torch.autograd.grad(0.3 * bal.balance + 0.01 * bal.z, x)                 # weights unused
+        only = ops.router_balance_bwd(d_l, x.detach(), coef, mask, off, None, None, None, score == "sigmoid")
+        assert torch.equal(got, only)
+        finished = F.balance_loss(x, e, score=score, **where)
+        assert torch.equal(finished.losses, losses)
+        assert torch.equal(torch.autograd.grad(finished.losses, x, d_l)[0], only)
+        assert torch.equal(torch.autograd.grad(ops.router_balance(x, e, mask, off, None, score == "sigmoid")[0], x, d_l)[0], only)
+    experts, weights, _ = F.route_balanced(x, 4)                                         # losses unused
+    got, = torch.autograd.grad(weights, x, d_w)
+    assert (got - ops.router_topk_bwd(experts, weights.detach(), d_w, 40)).abs().max() < 1e-6
+    y = x.detach().clone()
+    y[5] = np.nan                                                                        # and then not read for them
+    y.requires_grad_(True)
+    got, = torch.autograd.grad(F.route_balanced(y, 4)[1][:5], y, d_w[:5])
+    assert torch.isfinite(got[:5]).all() and bool((got[6:] == 0).all())
+
+
+def test_finished_counts_of_two_ranks_give_the_global_loss(cuda_device):
+    """Averaged over ranks, the loss with the summed counts is the loss of the whole batch."""
+    from mok import ops
+    logits = make(cuda_device, 800, 16, 2, seed=3)[0].to(cuda_device)
+    experts = ops.router_topk(logits, 2)[0]
+    whole, counts, _ = ops.router_balance(logits, experts)
+    halves = [(logits[a:a + 400], experts[a:a + 400]) for a in (0, 400)]
+    load = sum(ops.expert_counts(e, 16) for _, e in halves)
+    assert torch.equal(load, counts)
+    parts = [ops.router_balance(l, e, None, None, load)[0] for l, e in halves]
+    assert (sum(parts) / 2 - whole).abs().max() <= 2 * LOSS * float(whole.max())
+
+
+def test_group_of_one_rank(cuda_device, single_rank_group):
+    from mok import functional as F
+    x = make(cuda_device, 300, 24, 3, seed=3)[0].to(cuda_device).requires_grad_(True)
+    a, b = F.route_balanced(x, 3), F.route_balanced(x, 3, group=single_rank_group)
+    assert torch.equal(a[2].losses, b[2].losses) and torch.equal(a[2].counts, b[2].counts)
+    grads = [torch.autograd.grad([r[1].square().sum(), r[2].balance], x)[0] for r in (a, b)]
+    assert (grads[0] - grads[1]).abs().max() <= GRAD * 4
+
+
+def test_runs_and_streams_give_the_same_bytes(cuda_device):
+    from mok import ops
+    logits, where = make(cuda_device, 30000, 200, 6, S=11, mask=True, seed=2)
+    x, where = logits.to(cuda_device), on(cuda_device, where)
+    args = (x, 6, where["token_mask"], where["sequence_offsets"])
+    first = ops.router_topk_balance(*args)
+    d = torch.ones(2, device=cuda_device)
+    grad = ops.router_balance_bwd(d, x, first[4], *args[2:])
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for s in streams:                                       # three calls in flight at once
+        with torch.cuda.stream(s):
+            for _ in range(4):
+                out = ops.router_topk_balance(*args)
+                outs.append((out, ops.router_balance_bwd(d, x, out[4], *args[2:])))
+    torch.cuda.synchronize()
+    for out, g in outs:
+        assert all(torch.equal(a, b) for a, b in zip(out, first)) and torch.equal(g, grad)
+
+
+def test_two_captured_graphs_share_nothing(cuda_device):
+    from mok import ops
+    x = [make(cuda_device, 2000, 64, 4, seed=s)[0].to(cuda_device) for s in (1, 2)]
+    off = torch.tensor([0, 700, 1900], dtype=torch.int32, device=cuda_device)
+    d = torch.ones(2, device=cuda_device)
+
+    def step(l):
+        out = ops.router_topk_balance(l, 4, None, off)
+        return (*out, ops.router_balance_bwd(d, l, out[4], None, off, out[0], out[1], torch.ones_like(out[1])), ops.expert_counts(out[0], 64, None, off))
+    want = [[t.clone() for t in step(l)] for l in x]
+    side = torch.cuda.Stream(cuda_device)
+    with torch.cuda.stream(side):
+        step(x[0])
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for l in x:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(step(l))
+        graphs.append(g)
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        graphs[0].replay()
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
