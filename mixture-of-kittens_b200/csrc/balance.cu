@@ -25,7 +25,6 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kRowThreads = kWarps * 32;
 constexpr int kMaxRowBlocks = 592;             // not read from the device: the order of the sums is the same on every GPU
-constexpr int kJoinThreads = 256;
 constexpr int kJoinCols = 32;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -59,6 +58,13 @@ struct Scratch {
 
 int row_blocks(int T) { return std::min(kMaxRowBlocks, (T + kWarps - 1) / kWarps); }
 
+// how rows of E values of `bytes` bytes at `base` can be read: chunks of eight (16 or 32 bytes), of four, or one by one
+int chunk_of(const void* base, int E, int bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+    if (E % 8 == 0 && at % (8 * bytes) == 0) return 8;
+    return E % 4 == 0 && at % (4 * bytes) == 0 ? 4 : 1;
+}
+
 struct BalanceParams {
     const void* logits;
     const long long* top_in;       // finished routes, or null: this launch chooses them
@@ -73,6 +79,7 @@ struct BalanceParams {
     int T, E, K, S;
     int rows_per_block, blocks;
     int sigmoid;
+    int chunk;                     // see chunk_of
     SlotHead* head;
     float* slot_p;
     int* slot_routes;
@@ -82,20 +89,117 @@ struct BalanceParams {
     unsigned* ticket;
 };
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Reductions over groups of kLanes neighbouring lanes; every lane of the warp takes part.
+template <int kLanes>
+__device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(kAll, v, off);
+    for (int off = kLanes / 2; off > 0; off >>= 1) v += __shfl_xor_sync(kAll, v, off);
     return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
+template <int kLanes>
+__device__ __forceinline__ float group_max(float v) {       // a NaN loses against any number
+    if constexpr (kLanes == 32) {
+        float m;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+        return m;
+    }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, off));
+    for (int off = kLanes / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, off));
     return v;
 }
+template <int kLanes>
+__device__ __forceinline__ int group_min(int v) {
+    if constexpr (kLanes == 32) return __reduce_min_sync(kAll, v);
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) v = min(v, __shfl_xor_sync(kAll, v, off));
+    return v;
+}
+
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void from_float(float v, float& out) { out = v; }
 __device__ __forceinline__ void from_float(float v, __nv_bfloat16& out) { out = __float2bfloat16_rn(v); }
+
+// n (4 or 8) values from / to memory on a boundary of n values
+template <int n> __device__ __forceinline__ void load_chunk(const float* p, float* v) {
+    if constexpr (n == 8) {
+        uint32_t r[8];
+        ld_global_256(p, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+    } else {
+        const float4 r = *reinterpret_cast<const float4*>(p);
+        v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+    }
+}
+template <int n> __device__ __forceinline__ void load_chunk(const __nv_bfloat16* p, float* v) {
+    uint32_t w[n / 2];
+    if constexpr (n == 8) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+    } else {
+        const uint2 r = *reinterpret_cast<const uint2*>(p);
+        w[0] = r.x; w[1] = r.y;
+    }
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) { const float2 t = unpack_bf16(w[i]); v[2 * i] = t.x; v[2 * i + 1] = t.y; }
+}
+template <int n> __device__ __forceinline__ void store_chunk(float* p, const float* v) {
+    if constexpr (n == 8)
+        st_global_256(p, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]), __float_as_uint(v[4]),
+                      __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+    else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+template <int n> __device__ __forceinline__ void store_chunk(__nv_bfloat16* p, const float* v) {
+    if constexpr (n == 8) *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+}
+
+// A row of E values: the group's lane l holds values l V .. l V + V - 1 (so the lowest expert among equals is the lowest lane's
+// first).  Values past E read as `fill`.
+template <int V, typename T>
+__device__ __forceinline__ void load_row(const T* row, int e0, int E, int chunk, float fill, float (&v)[V]) {
+    if constexpr (V >= 8) {
+        if (chunk == 8) {
+#pragma unroll
+            for (int j = 0; j < V; j += 8) {
+                if (e0 + j < E) load_chunk<8>(row + e0 + j, v + j);
+                else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[j + i] = fill;
+                }
+            }
+            return;
+        }
+    }
+    if (chunk >= 4) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            if (e0 + j < E) load_chunk<4>(row + e0 + j, v + j);
+            else { v[j] = fill; v[j + 1] = fill; v[j + 2] = fill; v[j + 3] = fill; }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = e0 + j < E ? to_float(row[e0 + j]) : fill;
+    }
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_row(T* row, int e0, int E, int chunk, const float (&v)[V]) {
+    if constexpr (V >= 8) {
+        if (chunk == 8) {
+#pragma unroll
+            for (int j = 0; j < V; j += 8) if (e0 + j < E) store_chunk<8>(row + e0 + j, v + j);
+            return;
+        }
+    }
+    if (chunk >= 4) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) if (e0 + j < E) store_chunk<4>(row + e0 + j, v + j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) if (e0 + j < E) from_float(v[j], row[e0 + j]);
+    }
+}
 
 // Sequence bounds as the kernels use them: inside [0, T] whatever the caller's array holds.
 __device__ __forceinline__ int seq_bound(const int* offsets, int s, int T) {
@@ -109,95 +213,121 @@ __device__ __forceinline__ int first_sequence(const int* offsets, int S, int row
     return lo;
 }
 
-// sigma(l) times a factor common to the row, exp(-min(m, 0)) with m the row's maximum: the sum over the row cannot
-// underflow, and the factor cancels in every quotient
-__device__ __forceinline__ float sigmoid_scaled(float l, float shift) {
-    return l >= 0.0f ? 1.0f / (1.0f + expf(-l)) : expf(l - shift) / (1.0f + expf(l));
+// 1 / (1 + exp(-l)), and 1 minus that
+__device__ __forceinline__ float sigmoid(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
+__device__ __forceinline__ float sigmoid_rest(float l) { return l > 80.0f ? __expf(-l) : __fdividef(1.0f, 1.0f + __expf(l)); }
+// sigma(l) times a factor common to the row whose maximum is m: exp(-m) where m is negative, so that the sum over the row
+// cannot underflow; the factor cancels in every quotient
+__device__ __forceinline__ float sigmoid_scaled(float l, float m) {
+    return m >= 0.0f ? (l < -80.0f ? 0.0f : sigmoid(l)) : __fdividef(__expf(l - (m == -INFINITY ? 0.0f : m)), 1.0f + __expf(l));
 }
-__device__ __forceinline__ float sigmoid_shift(float m) { return m == -INFINITY ? 0.0f : fminf(m, 0.0f); }
 
-// Softmax statistics, probabilities and softmax of one row.  v[j] is the logit of expert lane + 32 j.  q[j] = softmax,
-// p[j] = what the balance loss averages (the same for softmax scores); returns lse, 0 for a row without a finite logit.
-template <int kPerLane>
-__device__ __forceinline__ float row_probs(const float (&v)[kPerLane], int lane, int E, int sigmoid, float (&p)[kPerLane],
-                                           float (&q)[kPerLane]) {
-    float m = -INFINITY;
+// Of one row held by a group of kLanes lanes: q = softmax, p = what the balance loss averages (the same for softmax scores).
+// Returns the log of the sum of exponentials, 0 for a row without a logit above -inf.  Exponentials go through the hardware's
+// base-2 one, two roundings of a difference and 2^-22 relative, below what the sums over a row round away.
+template <int kLanes, int V>
+__device__ __forceinline__ float row_probs(const float (&v)[V], int sigmoid_scores, float (&p)[V], float (&q)[V]) {
+    float m = v[0];
 #pragma unroll
-    for (int j = 0; j < kPerLane; ++j) m = fmaxf(m, v[j]);
-    m = warp_max(m);
-    const float base = m == -INFINITY ? 0.0f : m;
+    for (int j = 1; j < V; ++j) m = fmaxf(m, v[j]);
+    m = group_max<kLanes>(m);
+    const float base = m > -INFINITY ? m : 0.0f;
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kPerLane; ++j) { q[j] = expf(v[j] - base); sum += q[j]; }      // lanes past E hold -inf: 0
-    sum = warp_sum(sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int j = 0; j < V; ++j) { q[j] = __expf(v[j] - base); sum += q[j]; }     // lanes past E hold -inf: 0
+    sum = group_sum<kLanes>(sum);
+    const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
 #pragma unroll
-    for (int j = 0; j < kPerLane; ++j) q[j] *= inv;
-    if (sigmoid) {
-        const float shift = sigmoid_shift(m);
+    for (int j = 0; j < V; ++j) q[j] *= inv;
+    if (sigmoid_scores) {
         float total = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) { p[j] = sigmoid_scaled(v[j], shift); total += p[j]; }
-        total = warp_sum(total);
-        const float inv_p = total == 0.0f ? 0.0f : 1.0f / total;
+        for (int j = 0; j < V; ++j) { p[j] = sigmoid_scaled(v[j], m); total += p[j]; }
+        total = group_sum<kLanes>(total);
+        const float inv_p = total == 0.0f ? 0.0f : __fdividef(1.0f, total);
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) p[j] *= inv_p;
+        for (int j = 0; j < V; ++j) p[j] *= inv_p;
     } else {
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) p[j] = q[j];
+        for (int j = 0; j < V; ++j) p[j] = q[j];
     }
-    return sum == 0.0f ? 0.0f : base + logf(sum);
+    return sum == 0.0f ? 0.0f : base + __logf(sum);
 }
 
-// The K largest logits of a row, descending, the lower expert first among equals; a NaN ranks with -inf.  Lane k keeps
-// the k-th (value, expert).
-template <int kPerLane>
-__device__ __forceinline__ void row_select(const float (&v)[kPerLane], int lane, int E, int K, float& my_val, int& my_idx) {
+// The two largest values a lane has left, the lower index first among equals; slot V: none above -inf (a NaN is never above
+// anything, so it ranks with -inf).
+template <int V>
+__device__ __forceinline__ void two_largest(const float (&v)[V], unsigned taken, float& b1, int& j1, float& b2, int& j2) {
+    b1 = b2 = -INFINITY;
+    j1 = j2 = V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float x = (taken >> j) & 1u ? -INFINITY : v[j];
+        const bool first = x > b1, second = x > b2;
+        b2 = first ? b1 : second ? x : b2;
+        j2 = first ? j1 : second ? j : j2;
+        b1 = first ? x : b1;
+        j1 = first ? j : j1;
+    }
+}
+
+// The K largest values of a row, descending, the lower expert first among equals, into val / idx (shared memory of the group).
+// Every lane keeps the two largest values it has left; a round is one maximum over the group, the winner moves its second up,
+// and a lane that has used up both looks through its values again.  (With K = 8 of 256 over 32 lanes that happens in half
+// of the rows; one kept value would mean a search in every round.)
+template <int kLanes, int V>
+__device__ __forceinline__ void row_select(const float (&v)[V], int E, int K, float* val, int* idx) {
+    const int lane = threadIdx.x & 31, l = lane % kLanes;
+    const unsigned group = kLanes == 32 ? kAll : ((1u << kLanes) - 1u) << (lane - l);
+    const unsigned below = (1u << lane) - 1u;
+    const int mine = min(max(E - l * V, 0), V);                   // values of this lane that are there
     unsigned taken = 0;
-    my_val = -INFINITY;
-    my_idx = 0;
+    float b1, b2;
+    int j1, j2;
+    two_largest(v, 0u, b1, j1, b2, j2);
     for (int k = 0; k < K; ++k) {
-        float best = -INFINITY;
-        int best_e = 0x7fffffff;
-#pragma unroll
-        for (int j = 0; j < kPerLane; ++j) {
-            const int e = lane + 32 * j;
-            const float lv = v[j] == v[j] ? v[j] : -INFINITY;
-            if (e < E && !((taken >> j) & 1u) && (lv > best || best_e == 0x7fffffff)) { best = lv; best_e = e; }
+        const float best = group_max<kLanes>(b1);
+        const unsigned at = __ballot_sync(kAll, j1 < V && b1 == best) & group;
+        bool dry = false;
+        if (at & (1u << lane) && !(at & below)) {
+            val[k] = best;
+            idx[k] = l * V + j1;
+            taken |= 1u << j1;
+            b1 = b2; j1 = j2;
+            b2 = -INFINITY; j2 = V;
+            dry = j1 == V;
         }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-            const float ov = __shfl_xor_sync(kAll, best, off);
-            const int oe = __shfl_xor_sync(kAll, best_e, off);
-            if (oe != 0x7fffffff && (best_e == 0x7fffffff || ov > best || (ov == best && oe < best_e))) { best = ov; best_e = oe; }
+        if (__any_sync(kAll, at == 0)) {                           // nothing above -inf left: the lowest experts not taken yet
+            const unsigned left = ~taken & (V == 32 && mine == 32 ? kAll : (1u << mine) - 1u);
+            const int e = left ? l * V + __ffs(left) - 1 : 0x7fffffff;
+            const int lowest = group_min<kLanes>(e);
+            if (at == 0 && e == lowest && left) { val[k] = -INFINITY; idx[k] = e; taken |= left & (0u - left); }
         }
-        if ((best_e & 31) == lane) taken |= 1u << (best_e >> 5);
-        if (lane == k) { my_val = best; my_idx = best_e; }
+        if (__any_sync(kAll, dry)) { if (dry) two_largest(v, taken, b1, j1, b2, j2); }
     }
+    __syncwarp();
 }
 
-template <typename T, int kPerLane>
-__device__ __forceinline__ void load_row(const void* logits, size_t row, int lane, int E, float (&v)[kPerLane]) {
-    const T* at = static_cast<const T*>(logits) + row * E;
-#pragma unroll
-    for (int j = 0; j < kPerLane; ++j) { const int e = lane + 32 * j; v[j] = e < E ? to_float(at[e]) : -INFINITY; }
-}
-
-// HBM- or latency-bound: reads T E logits once, writes K routes a row and (p, routes) per slot.
-template <typename T, int kPerLane>
+// Bound by instructions: about 250 a row of 256 experts with eight routes, half of them for the choice.  Reads T E logits
+// once, writes K routes a row and (p, routes) per slot.
+template <typename T, int kLanes, int V>
 __global__ void __launch_bounds__(kRowThreads) balance_rows_kernel(const BalanceParams g) {
-    extern __shared__ float smem[];                        // p [kWarps][E], routes [E]
+    constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
+    extern __shared__ float smem[];                            // p [kWarps][E], routes [E], then the chosen values and experts [kGroups][K]
     __shared__ float s_z[kWarps];
     __shared__ int s_rows[kWarps], s_routes;
     int* const hist = reinterpret_cast<int*>(smem + static_cast<size_t>(kWarps) * g.E);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes;
+    float* const val = reinterpret_cast<float*>(hist + g.E) + static_cast<size_t>(group) * g.K;
+    int* const idx = hist + g.E + static_cast<size_t>(kGroups + group) * g.K;
+    const int e0 = l * V;
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
     const bool select = g.top_in == nullptr;
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
-    int s = first_sequence(g.offsets, g.S, pos, g.T);
+    int s = g.offsets == nullptr ? 0 : first_sequence(g.offsets, g.S, pos, g.T);
     while (pos < hi) {
         // the next run of rows: a sequence's, or rows between and behind the sequences
         const int begin = s < g.S ? max(seq_bound(g.offsets, s, g.T), pos) : hi;
@@ -209,37 +339,45 @@ __global__ void __launch_bounds__(kRowThreads) balance_rows_kernel(const Balance
             if (threadIdx.x == 0) s_routes = 0;
             __syncthreads();
         }
-        float acc[kPerLane], z = 0.0f;
+        float acc[V], z = 0.0f;
         int rows = 0, routes = 0;
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) acc[j] = 0.0f;
-        for (int t = pos + warp; t < end && (counted || select); t += kWarps) {
-            float v[kPerLane];
-            load_row<T>(g.logits, t, lane, g.E, v);
-            const bool live = counted && (g.mask == nullptr || g.mask[t]);
-            if (live) {
-                float p[kPerLane], q[kPerLane];
-                const float lse = row_probs(v, lane, g.E, g.sigmoid, p, q);
+        for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+        // all lanes of a warp stay in step; groups past the run work on nothing
+        for (int t0 = pos + warp * (32 / kLanes); t0 < end && (counted || select); t0 += kGroups) {
+            const int t = t0 + lane / kLanes;
+            const bool there = t < end;
+            float v[V];
+            load_row<V>(static_cast<const T*>(g.logits) + static_cast<size_t>(there ? t : t0) * g.E, e0, g.E, g.chunk, -INFINITY, v);
+            const bool live = there && counted && (g.mask == nullptr || g.mask[t]);
+            if (counted) {
+                float p[V], q[V];
+                const float lse = row_probs<kLanes>(v, g.sigmoid, p, q);
+                if (live) {
 #pragma unroll
-                for (int j = 0; j < kPerLane; ++j) acc[j] += p[j];
-                z += lse * lse;
-                ++rows;
+                    for (int j = 0; j < V; ++j) acc[j] += p[j];
+                    z += lse * lse;
+                    ++rows;
+                }
             }
             const size_t o = static_cast<size_t>(t) * g.K;
             if (select) {
-                float val; int idx;
-                row_select(v, lane, g.E, g.K, val, idx);
-                const float top = __shfl_sync(kAll, val, 0);
-                float w = 0.0f;
-                if (lane < g.K && top != -INFINITY) w = g.sigmoid ? sigmoid_scaled(val, sigmoid_shift(top)) : expf(val - top);
-                const float sum = warp_sum(w);
-                if (lane < g.K) {
-                    g.top_out[o + lane] = idx;
-                    g.weights[o + lane] = sum == 0.0f ? 0.0f : w / sum;
-                    if (live) { atomicAdd(&hist[idx], 1); ++routes; }
+                row_select<kLanes>(v, g.E, g.K, val, idx);
+                const float top = val[0];
+                float sum = 0.0f;
+                for (int k = l; k < g.K; k += kLanes)
+                    sum += top == -INFINITY ? 0.0f : g.sigmoid ? sigmoid_scaled(val[k], top) : __expf(val[k] - top);
+                sum = group_sum<kLanes>(sum);
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                for (int k = l; k < g.K && there; k += kLanes) {
+                    const float w = top == -INFINITY ? 0.0f : g.sigmoid ? sigmoid_scaled(val[k], top) : __expf(val[k] - top);
+                    g.top_out[o + k] = idx[k];
+                    g.weights[o + k] = w * inv;
+                    if (live) { atomicAdd(&hist[idx[k]], 1); ++routes; }
                 }
+                __syncwarp();
             } else if (live) {
-                for (int k = lane; k < g.K; k += 32) {
+                for (int k = l; k < g.K; k += kLanes) {
                     const long long e = g.top_in[o + k];
                     if (e >= 0 && e < g.E) { atomicAdd(&hist[e], 1); ++routes; }
                 }
@@ -248,7 +386,13 @@ __global__ void __launch_bounds__(kRowThreads) balance_rows_kernel(const Balance
         if (counted) {
             float* const mine = smem + static_cast<size_t>(warp) * g.E;
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) { const int e = lane + 32 * j; if (e < g.E) mine[e] = acc[j]; }
+            for (int j = 0; j < V; ++j) {
+#pragma unroll
+                for (int off = kLanes; off < 32; off <<= 1) acc[j] += __shfl_xor_sync(kAll, acc[j], off);
+                if (lane < kLanes && e0 + j < g.E) mine[e0 + j] = acc[j];
+            }
+#pragma unroll
+            for (int off = kLanes; off < 32; off <<= 1) { z += __shfl_xor_sync(kAll, z, off); rows += __shfl_xor_sync(kAll, rows, off); }
             if (routes) atomicAdd(&s_routes, routes);
             if (lane == 0) { s_z[warp] = z; s_rows[warp] = rows; }
             __syncthreads();
@@ -272,77 +416,66 @@ __global__ void __launch_bounds__(kRowThreads) balance_rows_kernel(const Balance
     }
 }
 
-template <typename V>
-__device__ __forceinline__ V block_sum(V v, V* tmp) {      // the same order on every run
-    tmp[threadIdx.x] = v;
-    __syncthreads();
-    for (int n = kJoinThreads / 2; n > 0; n >>= 1) {
-        if (threadIdx.x < n) tmp[threadIdx.x] += tmp[threadIdx.x + n];
-        __syncthreads();
-    }
-    const V sum = tmp[0];
-    __syncthreads();
-    return sum;
-}
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(kAll, v); }
 
-// One block per 32 experts of a sequence: adds the sequence's slots in block order; the block that finishes last adds up
-// the losses.
-__global__ void __launch_bounds__(kJoinThreads) balance_join_kernel(const BalanceParams g) {
-    __shared__ float tmp[kJoinThreads];
-    __shared__ int itmp[kJoinThreads];
+// One block per 32 experts of a sequence, one lane per expert; its warps take the sequence's slots in turn, and their sums
+// are added in warp order.  The block that finishes last adds up the losses.  Latency-bound: a few hundred slots at most.
+template <int kJoinWarps>
+__global__ void __launch_bounds__(kJoinWarps * 32) balance_join_kernel(const BalanceParams g) {
+    __shared__ float s_p[kJoinWarps][kJoinCols], s_z[kJoinWarps], s_balance[kJoinWarps];
+    __shared__ int s_c[kJoinWarps][kJoinCols], s_rows[kJoinWarps], s_routes[kJoinWarps];
     __shared__ bool last;
     pdl_wait();
     const int tiles = (g.E + kJoinCols - 1) / kJoinCols;
     const int s = blockIdx.x / tiles, tile = blockIdx.x - s * tiles;
     const int begin = seq_bound(g.offsets, s, g.T), end = seq_bound(g.offsets, s + 1, g.T);
     const int b0 = begin / g.rows_per_block, b1 = end > begin ? (end - 1) / g.rows_per_block + 1 : b0;
-    const int tid = threadIdx.x;
-    float z = 0.0f;
-    int rows = 0, routes = 0;
-    for (int b = b0 + tid; b < b1; b += kJoinThreads) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = tile * kJoinCols + lane;
+    float p = 0.0f, z = 0.0f;
+    int c = 0, rows = 0, routes = 0;
+#pragma unroll 4
+    for (int b = b0 + warp; b < b1; b += kJoinWarps) {
         const SlotHead h = g.head[b + s];
         z += h.z; rows += h.rows; routes += h.routes;
-    }
-    rows = block_sum(rows, itmp);
-    if (g.load != nullptr) {
-        routes = 0;
-        for (int e = tid; e < g.E; e += kJoinThreads) routes += g.load[static_cast<size_t>(s) * g.E + e];
-    }
-    routes = block_sum(routes, itmp);
-    z = block_sum(z, tmp);
-    const int col = tid % kJoinCols, r = tid / kJoinCols, e = tile * kJoinCols + col;
-    float p = 0.0f;
-    int c = 0;
-    if (e < g.E)
-        for (int b = b0 + r; b < b1; b += kJoinThreads / kJoinCols) {
+        if (e < g.E) {
             const size_t at = static_cast<size_t>(b + s) * g.E + e;
             p += g.slot_p[at];
             c += g.slot_routes[at];
         }
-    tmp[tid] = p;
-    itmp[tid] = c;
-    __syncthreads();
-    float part = 0.0f;
-    if (r == 0 && e < g.E) {
-        for (int i = 1; i < kJoinThreads / kJoinCols; ++i) { p += tmp[i * kJoinCols + col]; c += itmp[i * kJoinCols + col]; }
-        const size_t at = static_cast<size_t>(s) * g.E + e;
-        g.counts[at] = c;
-        const int used = g.load != nullptr ? g.load[at] : c;
-        const float f = static_cast<float>(g.E) * static_cast<float>(used) / static_cast<float>(max(routes, 1));
-        const float a = rows > 0 ? f / static_cast<float>(rows) : 0.0f;
-        g.coef[at] = a;
-        part = a * p;
     }
-    if (r == 0) {
-        part = warp_sum(part);
-        if (col == 0) {
+    s_p[warp][lane] = p;
+    s_c[warp][lane] = c;
+    if (lane == 0) { s_z[warp] = z; s_rows[warp] = rows; s_routes[warp] = routes; }
+    __syncthreads();
+    if (warp == 0) {
+        if (lane < kJoinWarps) { z = s_z[lane]; rows = s_rows[lane]; routes = s_routes[lane]; } else { z = 0.0f; rows = 0; routes = 0; }
+        z = group_sum<32>(z);
+        rows = warp_sum(rows);
+        if (g.load != nullptr) {
+            routes = 0;
+            for (int i = lane; i < g.E; i += 32) routes += g.load[static_cast<size_t>(s) * g.E + i];
+        }
+        routes = warp_sum(routes);
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w) { p += s_p[w][lane]; c += s_c[w][lane]; }
+        float part = 0.0f;
+        if (e < g.E) {
+            const size_t at = static_cast<size_t>(s) * g.E + e;
+            g.counts[at] = c;
+            const int used = g.load != nullptr ? g.load[at] : c;
+            const float f = static_cast<float>(g.E) * static_cast<float>(used) / static_cast<float>(max(routes, 1));
+            const float a = rows > 0 ? f / static_cast<float>(rows) : 0.0f;
+            g.coef[at] = a;
+            part = a * p;
+        }
+        part = group_sum<32>(part);
+        if (lane == 0) {
             g.part[blockIdx.x] = part;
             if (tile == 0) { g.seq_z[s] = z; g.seq_rows[s] = rows; }
+            __threadfence();
+            last = atomicAdd(g.ticket, 1u) == gridDim.x - 1;
         }
     }
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) last = atomicAdd(g.ticket, 1u) == gridDim.x - 1;
     __syncthreads();
     if (!last) return;
     __threadfence();
@@ -350,13 +483,16 @@ __global__ void __launch_bounds__(kJoinThreads) balance_join_kernel(const Balanc
     z = 0.0f;
     int live = 0;
     rows = 0;
-    for (int i = tid; i < static_cast<int>(gridDim.x); i += kJoinThreads) balance += __ldcg(&g.part[i]);
-    for (int i = tid; i < g.S; i += kJoinThreads) { const int n = __ldcg(&g.seq_rows[i]); z += __ldcg(&g.seq_z[i]); rows += n; live += n > 0; }
-    balance = block_sum(balance, tmp);
-    z = block_sum(z, tmp);
-    rows = block_sum(rows, itmp);
-    live = block_sum(live, itmp);
-    if (tid == 0) {
+    for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kJoinWarps * 32) balance += __ldcg(&g.part[i]);
+    for (int i = threadIdx.x; i < g.S; i += kJoinWarps * 32) { const int n = __ldcg(&g.seq_rows[i]); z += __ldcg(&g.seq_z[i]); rows += n; live += n > 0; }
+    balance = group_sum<32>(balance);
+    z = group_sum<32>(z);
+    rows = warp_sum(rows);
+    live = warp_sum(live);
+    if (lane == 0) { s_balance[warp] = balance; s_z[warp] = z; s_rows[warp] = rows; s_routes[warp] = live; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kJoinWarps; ++w) { balance += s_balance[w]; z += s_z[w]; rows += s_rows[w]; live += s_routes[w]; }
         const float n = static_cast<float>(max(rows, 1)), sequences = static_cast<float>(max(live, 1));
         g.losses[0] = balance / sequences;
         g.losses[1] = z / n;
@@ -375,59 +511,103 @@ struct BalanceBwdParams {
     const float* weights;
     const float* d_weights;
     void* d_logits;
-    int T, E, K, S, sigmoid;
+    int T, E, K, S, sigmoid, rows_per_block;
+    int chunk, coef_chunk;         // see chunk_of: for the logits and their gradient, and for coef
 };
 
-// One warp per row; reads and writes T E values.
-template <typename T, int kPerLane>
+// Bound by DRAM at large sizes: reads T E logits, writes T E gradients.  The gradient of the chosen weights is scattered into a
+// row of shared memory, K values, and picked up by the lanes that hold their experts.
+template <typename T, int kLanes, int V>
 __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceBwdParams g) {
-    const int lane = threadIdx.x & 31;
+    constexpr int kGroups = kRowThreads / kLanes;
+    __shared__ alignas(16) float s_add[kGroups][kLanes * V];
+    const int lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes, e0 = l * V;
+    float* const add = s_add[group];
+#pragma unroll
+    for (int j = 0; j < V; ++j) add[e0 + j] = 0.0f;
     pdl_wait();
     const size_t scalars = static_cast<size_t>(g.S) * g.E;
     const float gb = g.d_losses[0] * g.coef[scalars], gz = g.d_losses[1] * g.coef[scalars + 1];
-    for (long long t = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < g.T;
-         t += static_cast<long long>(gridDim.x) * kWarps) {
-        float d[kPerLane];
+    const bool losses = gb != 0.0f || gz != 0.0f;      // without an upstream gradient the row is not read for them
+    const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
+    const int lo = static_cast<int>(min(first, static_cast<long long>(g.T)));
+    const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
+    int s = g.offsets == nullptr ? 0 : first_sequence(g.offsets, g.S, lo, g.T), held = -1;
+    float a[V];
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) d[j] = 0.0f;
-        const int s = first_sequence(g.offsets, g.S, static_cast<int>(t), g.T);
-        // without an upstream gradient of the losses the row is not read for them (nothing times NaN stays nothing)
-        const bool live = (gb != 0.0f || gz != 0.0f) && s < g.S && seq_bound(g.offsets, s, g.T) <= t && (g.mask == nullptr || g.mask[t]);
-        if (live) {
-            float v[kPerLane], p[kPerLane], q[kPerLane];
-            load_row<T>(g.logits, t, lane, g.E, v);
-            const float lse = row_probs(v, lane, g.E, g.sigmoid, p, q);
-            const float* a = g.coef + static_cast<size_t>(s) * g.E;
-            float av[kPerLane], dot = 0.0f;
+    for (int j = 0; j < V; ++j) a[j] = 0.0f;
+    __syncwarp();
+    for (int t0 = lo + (threadIdx.x >> 5) * (32 / kLanes); t0 < hi; t0 += kGroups) {
+        const int t = t0 + lane / kLanes;
+        const bool there = t < hi;
+        bool live = there && losses && (g.mask == nullptr || g.mask[t]);
+        if (g.offsets != nullptr && there) {
+            while (s < g.S && seq_bound(g.offsets, s + 1, g.T) <= t) ++s;
+            live = live && s < g.S && seq_bound(g.offsets, s, g.T) <= t;
+        }
+        if (live && s != held) {
+            load_row<V>(g.coef + static_cast<size_t>(s) * g.E, e0, g.E, g.coef_chunk, 0.0f, a);
+            held = s;
+        }
+        float d[V], v[V];
+        const T* const row = static_cast<const T*>(g.logits) + static_cast<size_t>(there ? t : t0) * g.E;
+        if (losses) {
+            float p[V], q[V];
+            load_row<V>(row, e0, g.E, g.chunk, -INFINITY, v);
+            const float lse = row_probs<kLanes>(v, g.sigmoid, p, q);
+            float dot = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) { const int e = lane + 32 * j; av[j] = e < g.E ? a[e] : 0.0f; dot += p[j] * av[j]; }
-            dot = warp_sum(dot);
+            for (int j = 0; j < V; ++j) dot += p[j] * a[j];
+            dot = group_sum<kLanes>(dot);
+            const float zs = gz * lse;
 #pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
-                float slope = p[j] * (av[j] - dot);
-                if (g.sigmoid) slope /= 1.0f + expf(v[j]);
-                d[j] = gb * slope + gz * lse * q[j];
+            for (int j = 0; j < V; ++j) {
+                float slope = p[j] * (a[j] - dot);
+                if (g.sigmoid) slope *= sigmoid_rest(v[j]);
+                d[j] = live ? gb * slope + zs * q[j] : 0.0f;
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) d[j] = 0.0f;
         }
         if (g.top != nullptr) {
-            const size_t o = static_cast<size_t>(t) * g.K + lane;
-            const float w = lane < g.K ? g.weights[o] : 0.0f, dw = lane < g.K ? g.d_weights[o] : 0.0f;
-            const long long top = lane < g.K ? g.top[o] : -1;
-            const int idx = top >= 0 && top < g.E ? static_cast<int>(top) : -1;
-            const float dot = warp_sum(w * dw);
-            float add = w * (dw - dot);
-            if (g.sigmoid && idx >= 0) add /= 1.0f + expf(to_float(static_cast<const T*>(g.logits)[static_cast<size_t>(t) * g.E + idx]));
-            if (w == 0.0f) add = 0.0f;
-            for (int k = 0; k < g.K; ++k) {
-                const int e = __shfl_sync(kAll, idx, k);
-                const float x = __shfl_sync(kAll, add, k);
-#pragma unroll
-                for (int j = 0; j < kPerLane; ++j) if (e == lane + 32 * j) d[j] += x;
+            const size_t o = static_cast<size_t>(t) * g.K;
+            float dot = 0.0f;
+            for (int k = l; k < g.K && there; k += kLanes) dot += g.weights[o + k] * g.d_weights[o + k];
+            dot = group_sum<kLanes>(dot);
+            auto expert = [&](int k) { const long long e = g.top[o + k]; return e >= 0 && e < g.E ? static_cast<int>(e) : -1; };
+            auto value = [&](int k, int e) {
+                const float w = g.weights[o + k];
+                float x = w * (g.d_weights[o + k] - dot);
+                if (g.sigmoid) x *= sigmoid_rest(to_float(row[e]));
+                return w == 0.0f ? 0.0f : x;
+            };
+            // an expert that a row names twice (finished routes may) shows in the tag that was overwritten
+            bool twice = false;
+            for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = __int_as_float(k); }
+            __syncwarp();
+            for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); twice |= e >= 0 && __float_as_int(add[e]) != k; }
+            if (__any_sync(kAll, twice)) {
+                for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = 0.0f; }
+                for (int k = 0; k < g.K; ++k) {                   // one at a time, in order
+                    __syncwarp();
+                    if (there && k % kLanes == l) { const int e = expert(k); if (e >= 0) add[e] += value(k, e); }
+                }
+            } else {
+                __syncwarp();
+                for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = value(k, e); }
             }
-        }
-        T* out = static_cast<T*>(g.d_logits) + static_cast<size_t>(t) * g.E;
+            __syncwarp();
 #pragma unroll
-        for (int j = 0; j < kPerLane; ++j) { const int e = lane + 32 * j; if (e < g.E) from_float(d[j], out[e]); }
+            for (int j = 0; j < V; j += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(add + e0 + j);
+                d[j] += x.x; d[j + 1] += x.y; d[j + 2] += x.z; d[j + 3] += x.w;
+            }
+            __syncwarp();
+            for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = 0.0f; }
+            __syncwarp();
+        }
+        if (there) store_row<V>(static_cast<T*>(g.d_logits) + static_cast<size_t>(t) * g.E, e0, g.E, g.chunk, d);
     }
 }
 
@@ -468,27 +648,30 @@ __global__ void __launch_bounds__(kRowThreads) expert_counts_kernel(const CountP
     }
 }
 
-template <typename T, int kPerLane>
+template <typename T, int kLanes, int V>
 int launch_rows(const BalanceParams& p, cudaStream_t s) {
-    const size_t smem = static_cast<size_t>(kWarps + 1) * p.E * 4;
-    return launch_kernel(balance_rows_kernel<T, kPerLane>, p.blocks, kRowThreads, smem, s, false, false, p);
+    const size_t chosen = p.top_in == nullptr ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
+    return launch_kernel(balance_rows_kernel<T, kLanes, V>, p.blocks, kRowThreads, (static_cast<size_t>(kWarps + 1) * p.E + chosen) * 4, s, false, true, p);
 }
 
-template <typename T, int kPerLane>
-int launch_bwd(const BalanceBwdParams& p, cudaStream_t s) {
-    const int blocks = std::min((p.T + kWarps - 1) / kWarps, device_sm_count() * 8);
-    return launch_kernel(balance_bwd_kernel<T, kPerLane>, blocks, kRowThreads, 0, s, false, false, p);
+template <typename T, int kLanes, int V>
+int launch_bwd(BalanceBwdParams p, cudaStream_t s) {
+    constexpr int kGroups = kRowThreads / kLanes;
+    const int blocks = std::min((p.T + kGroups - 1) / kGroups, device_sm_count() * 8);
+    p.rows_per_block = (p.T + blocks - 1) / blocks;
+    return launch_kernel(balance_bwd_kernel<T, kLanes, V>, blocks, kRowThreads, 0, s, false, true, p);
 }
 
-#define MOK_PER_LANE(call)                                                                       \
+// lanes a row and values a lane: four values where a row fits, so that 32 lanes hold several short rows
+#define MOK_ROW_SHAPE(E, call)                                                                   \
     [&] {                                                                                        \
-        const int per_lane = (p.E + 31) / 32;                                                    \
-        if (per_lane <= 1) return call(1);                                                       \
-        if (per_lane <= 2) return call(2);                                                       \
-        if (per_lane <= 4) return call(4);                                                       \
-        if (per_lane <= 8) return call(8);                                                       \
-        if (per_lane <= 16) return call(16);                                                     \
-        return call(32);                                                                         \
+        if ((E) <= 16) return call(4, 4);                                                        \
+        if ((E) <= 32) return call(8, 4);                                                        \
+        if ((E) <= 64) return call(16, 4);                                                       \
+        if ((E) <= 128) return call(32, 4);                                                      \
+        if ((E) <= 256) return call(32, 8);                                                      \
+        if ((E) <= 512) return call(32, 16);                                                     \
+        return call(32, 32);                                                                     \
     }()
 
 bool bad_sizes(int T, int E, int K, int S) { return T <= 0 || E <= 0 || K <= 0 || K > 255 || S <= 0; }
@@ -532,22 +715,25 @@ extern "C" int mok_router_balance(const void* logits, int logits_bf16, int num_t
     p.T = num_tokens; p.E = num_experts; p.K = topk; p.S = num_sequences;
     p.rows_per_block = (num_tokens + p.blocks - 1) / p.blocks;
     p.sigmoid = sigmoid;
+    p.chunk = chunk_of(logits, num_experts, logits_bf16 ? 2 : 4);
     p.head = at.head; p.slot_p = at.p; p.slot_routes = at.routes; p.part = at.part; p.seq_z = at.seq_z; p.seq_rows = at.seq_rows;
     p.ticket = at.ticket;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(kSlotOther, s, 2);
     int rc;
     if (logits_bf16) {
-#define MOK_CALL(n) launch_rows<__nv_bfloat16, n>(p, s)
-        rc = MOK_PER_LANE(MOK_CALL);
+#define MOK_CALL(lanes, v) launch_rows<__nv_bfloat16, lanes, v>(p, s)
+        rc = MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
     } else {
-#define MOK_CALL(n) launch_rows<float, n>(p, s)
-        rc = MOK_PER_LANE(MOK_CALL);
+#define MOK_CALL(lanes, v) launch_rows<float, lanes, v>(p, s)
+        rc = MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
     }
     if (rc != MOK_OK) return rc;
-    return launch_kernel(balance_join_kernel, num_sequences * tiles, kJoinThreads, 0, s, false, false, p);
+    // warps for the slots of a sequence, on average
+    if (p.blocks / num_sequences >= 64) return launch_kernel(balance_join_kernel<32>, num_sequences * tiles, 1024, 0, s, false, true, p);
+    return launch_kernel(balance_join_kernel<8>, num_sequences * tiles, 256, 0, s, false, true, p);
 }
 
 extern "C" int mok_router_balance_bwd(const float* d_losses, const void* logits, int logits_bf16, const float* coef,
@@ -560,16 +746,18 @@ extern "C" int mok_router_balance_bwd(const float* d_losses, const void* logits,
     if (!sequence_offsets && num_sequences != 1) return MOK_ERR_INVALID;
     if (num_experts > 1024) return MOK_ERR_UNSUPPORTED;
     BalanceBwdParams p{d_losses, logits, coef, token_mask, sequence_offsets, reinterpret_cast<const long long*>(top_experts),
-                       router_weights, d_router_weights, d_logits, num_tokens, num_experts, topk, num_sequences, sigmoid};
+                       router_weights, d_router_weights, d_logits, num_tokens, num_experts, topk, num_sequences, sigmoid, 0,
+                       std::min(chunk_of(logits, num_experts, logits_bf16 ? 2 : 4), chunk_of(d_logits, num_experts, logits_bf16 ? 2 : 4)),
+                       chunk_of(coef, num_experts, 4)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(kSlotOther, s);
     if (logits_bf16) {
-#define MOK_CALL(n) launch_bwd<__nv_bfloat16, n>(p, s)
-        return MOK_PER_LANE(MOK_CALL);
+#define MOK_CALL(lanes, v) launch_bwd<__nv_bfloat16, lanes, v>(p, s)
+        return MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
     }
-#define MOK_CALL(n) launch_bwd<float, n>(p, s)
-    return MOK_PER_LANE(MOK_CALL);
+#define MOK_CALL(lanes, v) launch_bwd<float, lanes, v>(p, s)
+    return MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
 }
 

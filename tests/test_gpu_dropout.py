@@ -199,7 +199,7 @@ def test_layer_without_the_new_arguments_is_what_it_was(cuda_device, single_rank
     layer, x, _, g = layer_and_inputs(cuda_device, single_rank_group)
     out = layer(x)
     withb, bal = layer(x, return_balance=True)
-    assert torch.equal(out, withb) or float((out.float() - withb.float()).abs().max()) <= 2.0 ** -7 * float(out.float().abs().max())
+    assert torch.equal(out, withb) or float((out.detach().float() - withb.detach().float()).abs().max()) <= 2.0 ** -7 * float(out.detach().float().abs().max())
     assert int(bal.counts.sum()) == 1024 * 2 and tuple(bal.counts.shape) == (1, 8)
 
 
