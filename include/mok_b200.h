@@ -173,7 +173,7 @@ int mok_router_topk_bwd(const int32_t* top_experts_i32, const float* router_weig
  * [num_sequences, E], coef f32 [num_sequences * E + 2] for mok_router_balance_bwd.  scratch: 16-byte aligned,
  * mok_router_balance_scratch_bytes bytes, of this call alone until it has run.
  * mok_router_balance_bwd writes all of d_logits (type of logits) from d_losses f32 [2] and, where the three are not NULL,
- * from the gradient of the router weights (topk <= 32).
+ * from the gradient of the router weights (topk <= 32 and <= num_experts).
  * No reference counterpart (the reference takes finished routes and returns no losses). */
 size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences);
 int mok_router_balance(const void* logits, int logits_bf16, int num_tokens, int num_experts, int topk, int num_sequences,

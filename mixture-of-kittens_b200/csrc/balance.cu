@@ -24,7 +24,9 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kRowThreads = kWarps * 32;
-constexpr int kMaxRowBlocks = 592;             // not read from the device: the order of the sums is the same on every GPU
+// Blocks of the forward pass, all resident at once on 148 SMs: four an SM up to 256 experts, two above (their rows take twice
+// the registers).  Not read from the device: the order of the sums is the same on every GPU.
+constexpr int row_blocks_per_sm(int E) { return E <= 256 ? 4 : 2; }
 constexpr int kJoinCols = 32;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -56,7 +58,7 @@ struct Scratch {
     }
 };
 
-int row_blocks(int T) { return std::min(kMaxRowBlocks, (T + kWarps - 1) / kWarps); }
+int row_blocks(int T, int E) { return std::min(148 * row_blocks_per_sm(E), (T + kWarps - 1) / kWarps); }
 
 // how rows of E values of `bytes` bytes at `base` can be read: chunks of eight (16 or 32 bytes), of four, or one by one
 int chunk_of(const void* base, int E, int bytes) {
@@ -213,45 +215,48 @@ __device__ __forceinline__ int first_sequence(const int* offsets, int S, int row
     return lo;
 }
 
-// 1 / (1 + exp(-l)), and 1 minus that
-__device__ __forceinline__ float sigmoid(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
-__device__ __forceinline__ float sigmoid_rest(float l) { return l > 80.0f ? __expf(-l) : __fdividef(1.0f, 1.0f + __expf(l)); }
+// Exponentials, logarithms and quotients go through the hardware's approximate base-2 ones, results below 2^-126 flushed to
+// zero: 2^-22 relative and the rounding of the argument, below what the sums over a row round away.  exp(v - m) is
+// 2^(v log2(e) - m log2(e)), one fused multiply-add.
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float rcp_fast(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float log_fast(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y * kLn2; }
+
 // sigma(l) times a factor common to the row whose maximum is m: exp(-m) where m is negative, so that the sum over the row
 // cannot underflow; the factor cancels in every quotient
 __device__ __forceinline__ float sigmoid_scaled(float l, float m) {
-    return m >= 0.0f ? (l < -80.0f ? 0.0f : sigmoid(l)) : __fdividef(__expf(l - (m == -INFINITY ? 0.0f : m)), 1.0f + __expf(l));
+    if (m >= 0.0f) return rcp_fast(1.0f + exp2_fast(-l * kLog2e));
+    return exp2_fast((l - (m > -INFINITY ? m : 0.0f)) * kLog2e) * rcp_fast(1.0f + exp2_fast(l * kLog2e));
 }
+__device__ __forceinline__ float sigmoid_rest(float l) { return rcp_fast(1.0f + exp2_fast(l * kLog2e)); }      // 1 - sigma(l)
 
-// Of one row held by a group of kLanes lanes: q = softmax, p = what the balance loss averages (the same for softmax scores).
-// Returns the log of the sum of exponentials, 0 for a row without a logit above -inf.  Exponentials go through the hardware's
-// base-2 one, two roundings of a difference and 2^-22 relative, below what the sums over a row round away.
-template <int kLanes, int V>
-__device__ __forceinline__ float row_probs(const float (&v)[V], int sigmoid_scores, float (&p)[V], float (&q)[V]) {
+// Of one row held by a group of kLanes lanes: ex = exponentials and inv the reciprocal of their sum (softmax = ex inv), for
+// sigmoid scores also sg = scaled sigmoids and inv_sg.  inv is 0 for a row without a logit above -inf, and lse then 0.
+struct RowStats { float inv, inv_sg, lse; };
+template <int kLanes, int V, bool kSigmoid>
+__device__ __forceinline__ RowStats row_stats(const float (&v)[V], float (&ex)[V], float (&sg)[V]) {
     float m = v[0];
 #pragma unroll
     for (int j = 1; j < V; ++j) m = fmaxf(m, v[j]);
     m = group_max<kLanes>(m);
-    const float base = m > -INFINITY ? m : 0.0f;
+    const float base = m > -INFINITY ? m : 0.0f, shift = -base * kLog2e;
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) { q[j] = __expf(v[j] - base); sum += q[j]; }     // lanes past E hold -inf: 0
+    for (int j = 0; j < V; ++j) { ex[j] = exp2_fast(fmaf(v[j], kLog2e, shift)); sum += ex[j]; }     // lanes past E hold -inf: 0
     sum = group_sum<kLanes>(sum);
-    const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
-#pragma unroll
-    for (int j = 0; j < V; ++j) q[j] *= inv;
-    if (sigmoid_scores) {
+    RowStats r;
+    r.inv = sum == 0.0f ? 0.0f : rcp_fast(sum);
+    r.lse = sum == 0.0f ? 0.0f : base + log_fast(sum);
+    r.inv_sg = 0.0f;
+    if constexpr (kSigmoid) {
         float total = 0.0f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) { p[j] = sigmoid_scaled(v[j], m); total += p[j]; }
+        for (int j = 0; j < V; ++j) { sg[j] = sigmoid_scaled(v[j], m); total += sg[j]; }
         total = group_sum<kLanes>(total);
-        const float inv_p = total == 0.0f ? 0.0f : __fdividef(1.0f, total);
-#pragma unroll
-        for (int j = 0; j < V; ++j) p[j] *= inv_p;
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = q[j];
+        r.inv_sg = total == 0.0f ? 0.0f : rcp_fast(total);
     }
-    return sum == 0.0f ? 0.0f : base + __logf(sum);
+    return r;
 }
 
 // The two largest values a lane has left, the lower index first among equals; slot V: none above -inf (a NaN is never above
@@ -271,12 +276,14 @@ __device__ __forceinline__ void two_largest(const float (&v)[V], unsigned taken,
     }
 }
 
-// The K largest values of a row, descending, the lower expert first among equals, into val / idx (shared memory of the group).
-// Every lane keeps the two largest values it has left; a round is one maximum over the group, the winner moves its second up,
-// and a lane that has used up both looks through its values again.  (With K = 8 of 256 over 32 lanes that happens in half
-// of the rows; one kept value would mean a search in every round.)
+// The K largest values of a row, descending, the lower expert first among equals, into chosen[0..K) (shared memory of the
+// group) as (value, expert).
+//
+// In rounds: every lane keeps the two largest values it has left; a round is one maximum over the group, the winner moves its
+// second up, and a lane that has used up both looks through its values again (with K = 8 of 256 over 32 lanes in half of
+// the rows; one kept value would mean a search in every round).
 template <int kLanes, int V>
-__device__ __forceinline__ void row_select(const float (&v)[V], int E, int K, float* val, int* idx) {
+__device__ __forceinline__ void select_in_rounds(const float (&v)[V], int E, int K, float2* chosen) {
     const int lane = threadIdx.x & 31, l = lane % kLanes;
     const unsigned group = kLanes == 32 ? kAll : ((1u << kLanes) - 1u) << (lane - l);
     const unsigned below = (1u << lane) - 1u;
@@ -287,39 +294,83 @@ __device__ __forceinline__ void row_select(const float (&v)[V], int E, int K, fl
     two_largest(v, 0u, b1, j1, b2, j2);
     for (int k = 0; k < K; ++k) {
         const float best = group_max<kLanes>(b1);
-        const unsigned at = __ballot_sync(kAll, j1 < V && b1 == best) & group;
-        bool dry = false;
-        if (at & (1u << lane) && !(at & below)) {
-            val[k] = best;
-            idx[k] = l * V + j1;
-            taken |= 1u << j1;
-            b1 = b2; j1 = j2;
-            b2 = -INFINITY; j2 = V;
-            dry = j1 == V;
-        }
+        const bool equal = j1 < V && b1 == best;
+        const unsigned at = __ballot_sync(kAll, equal) & group;
+        const bool win = equal && (at & below) == 0;
+        if (win) chosen[k] = make_float2(best, __int_as_float(l * V + j1));
+        taken |= win ? 1u << (j1 & 31) : 0u;
+        const bool dry = win && j2 == V;
+        b1 = win ? b2 : b1;
+        j1 = win ? j2 : j1;
+        b2 = win ? -INFINITY : b2;
+        j2 = win ? V : j2;
         if (__any_sync(kAll, at == 0)) {                           // nothing above -inf left: the lowest experts not taken yet
             const unsigned left = ~taken & (V == 32 && mine == 32 ? kAll : (1u << mine) - 1u);
             const int e = left ? l * V + __ffs(left) - 1 : 0x7fffffff;
             const int lowest = group_min<kLanes>(e);
-            if (at == 0 && e == lowest && left) { val[k] = -INFINITY; idx[k] = e; taken |= left & (0u - left); }
+            if (at == 0 && e == lowest && left) { chosen[k] = make_float2(-INFINITY, __int_as_float(e)); taken |= left & (0u - left); }
         }
         if (__any_sync(kAll, dry)) { if (dry) two_largest(v, taken, b1, j1, b2, j2); }
     }
     __syncwarp();
 }
 
-// Bound by instructions: about 250 a row of 256 experts with eight routes, half of them for the choice.  Reads T E logits
-// once, writes K routes a row and (p, routes) per slot.
-template <typename T, int kLanes, int V>
-__global__ void __launch_bounds__(kRowThreads) balance_rows_kernel(const BalanceParams g) {
+// One row a warp: with t the K-th largest of the lanes' maxima, at least K values are >= t and only few more; they are
+// gathered, one a lane, and every lane counts those that come before its own.  Rows where that does not work out (fewer than K
+// lanes with a value above -inf, more than 32 values >= t) go in rounds.  131072 rows of 256, K = 8, rounds -> this, forward:
+// see the figures at balance_rows_kernel.
+template <int V>
+__device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K, float2* gathered, float2* chosen) {
+    const int lane = threadIdx.x & 31;
+    float b = v[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) b = fmaxf(b, v[j]);
+    b = b > -INFINITY ? b : -INFINITY;                             // all NaN
+    float t;
+    int found = 0;
+    do {
+        t = group_max<32>(b);
+        const bool equal = b == t;
+        found += __popc(__ballot_sync(kAll, equal));
+        b = equal ? -INFINITY : b;
+    } while (found < K && t > -INFINITY);
+    int n = 0;
+    if (t > -INFINITY) {
+        const unsigned below = (1u << lane) - 1u;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = v[j] >= t;
+            const unsigned at = __ballot_sync(kAll, in);
+            const int to = n + __popc(at & below);
+            if (in && to < 32) gathered[to] = make_float2(v[j], __int_as_float(lane * V + j));
+            n += __popc(at);
+        }
+    }
+    if (t == -INFINITY || n > 32) { select_in_rounds<32, V>(v, E, K, chosen); return; }
+    __syncwarp();
+    const float2 mine = gathered[lane];                            // past n: left over, not used
+    const int e = __float_as_int(mine.y);
+    int before = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float2 other = gathered[i];
+        before += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
+    }
+    if (lane < n && before < K) chosen[before] = mine;
+    __syncwarp();
+}
+
+// Bound by instructions.  Reads T E logits once, writes K routes a row and (p, routes) per slot.
+template <typename T, int kLanes, int V, bool kSigmoid>
+__global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) balance_rows_kernel(const BalanceParams g) {
     constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
-    extern __shared__ float smem[];                            // p [kWarps][E], routes [E], then the chosen values and experts [kGroups][K]
+    extern __shared__ float smem[];                            // p [kWarps][E], routes [E], then the chosen (value, expert) [kGroups][K]
+    __shared__ float2 s_gathered[kWarps][32];
     __shared__ float s_z[kWarps];
     __shared__ int s_rows[kWarps], s_routes;
     int* const hist = reinterpret_cast<int*>(smem + static_cast<size_t>(kWarps) * g.E);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes;
-    float* const val = reinterpret_cast<float*>(hist + g.E) + static_cast<size_t>(group) * g.K;
-    int* const idx = hist + g.E + static_cast<size_t>(kGroups + group) * g.K;
+    float2* const chosen = reinterpret_cast<float2*>(hist + ((g.E + 1) & ~1)) + static_cast<size_t>(group) * g.K;
     const int e0 = l * V;
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
@@ -350,30 +401,34 @@ __global__ void __launch_bounds__(kRowThreads) balance_rows_kernel(const Balance
             float v[V];
             load_row<V>(static_cast<const T*>(g.logits) + static_cast<size_t>(there ? t : t0) * g.E, e0, g.E, g.chunk, -INFINITY, v);
             const bool live = there && counted && (g.mask == nullptr || g.mask[t]);
+            const size_t o = static_cast<size_t>(t) * g.K;
             if (counted) {
-                float p[V], q[V];
-                const float lse = row_probs<kLanes>(v, g.sigmoid, p, q);
+                float ex[V], sg[V];
+                const RowStats r = row_stats<kLanes, V, kSigmoid>(v, ex, sg);
                 if (live) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) acc[j] += p[j];
-                    z += lse * lse;
+                    for (int j = 0; j < V; ++j) acc[j] = kSigmoid ? fmaf(sg[j], r.inv_sg, acc[j]) : fmaf(ex[j], r.inv, acc[j]);
+                    z = fmaf(r.lse, r.lse, z);
                     ++rows;
                 }
             }
-            const size_t o = static_cast<size_t>(t) * g.K;
             if (select) {
-                row_select<kLanes>(v, g.E, g.K, val, idx);
-                const float top = val[0];
+                if constexpr (kLanes == 32) select_by_rank<V>(v, g.E, g.K, s_gathered[warp], chosen);
+                else select_in_rounds<kLanes, V>(v, g.E, g.K, chosen);
+                const float top = chosen[0].x;
+                auto weight = [&](float x) {
+                    return top == -INFINITY ? 0.0f : kSigmoid ? sigmoid_scaled(x, top) : exp2_fast((x - top) * kLog2e);
+                };
                 float sum = 0.0f;
-                for (int k = l; k < g.K; k += kLanes)
-                    sum += top == -INFINITY ? 0.0f : g.sigmoid ? sigmoid_scaled(val[k], top) : __expf(val[k] - top);
+                for (int k = l; k < g.K; k += kLanes) sum += weight(chosen[k].x);
                 sum = group_sum<kLanes>(sum);
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float inv = sum == 0.0f ? 0.0f : rcp_fast(sum);
                 for (int k = l; k < g.K && there; k += kLanes) {
-                    const float w = top == -INFINITY ? 0.0f : g.sigmoid ? sigmoid_scaled(val[k], top) : __expf(val[k] - top);
-                    g.top_out[o + k] = idx[k];
-                    g.weights[o + k] = w * inv;
-                    if (live) { atomicAdd(&hist[idx[k]], 1); ++routes; }
+                    const float2 c = chosen[k];
+                    const int e = __float_as_int(c.y);
+                    g.top_out[o + k] = e;
+                    g.weights[o + k] = weight(c.x) * inv;
+                    if (live) { atomicAdd(&hist[e], 1); ++routes; }
                 }
                 __syncwarp();
             } else if (live) {
@@ -515,11 +570,13 @@ struct BalanceBwdParams {
     int chunk, coef_chunk;         // see chunk_of: for the logits and their gradient, and for coef
 };
 
-// Bound by DRAM at large sizes: reads T E logits, writes T E gradients.  The gradient of the chosen weights is scattered into a
-// row of shared memory, K values, and picked up by the lanes that hold their experts.
-template <typename T, int kLanes, int V>
+// Bound by DRAM at large sizes: reads T E logits, writes T E gradients.  With c = gb (a - sum p a) + gz lse the softmax row's
+// gradient is p c: two operations a value once the sums are there.  The gradient of the chosen weights is scattered into a row
+// of shared memory, K values, and picked up by the lanes that hold their experts.
+template <typename T, int kLanes, int V, bool kSigmoid>
 __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceBwdParams g) {
     constexpr int kGroups = kRowThreads / kLanes;
+    constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // routes a lane, at most (topk <= 32 and <= E)
     __shared__ alignas(16) float s_add[kGroups][kLanes * V];
     const int lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes, e0 = l * V;
     float* const add = s_add[group];
@@ -533,13 +590,29 @@ __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceB
     const int lo = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
     int s = g.offsets == nullptr ? 0 : first_sequence(g.offsets, g.S, lo, g.T), held = -1;
-    float a[V];
+    float a[V];                                        // gb times the sequence's f / n
 #pragma unroll
     for (int j = 0; j < V; ++j) a[j] = 0.0f;
     __syncwarp();
     for (int t0 = lo + (threadIdx.x >> 5) * (32 / kLanes); t0 < hi; t0 += kGroups) {
         const int t = t0 + lane / kLanes;
         const bool there = t < hi;
+        const T* const row = static_cast<const T*>(g.logits) + static_cast<size_t>(there ? t : t0) * g.E;
+        float d[V], v[V];
+        if (losses) load_row<V>(row, e0, g.E, g.chunk, -INFINITY, v);
+        int expert[kPer];
+        float w[kPer], dw[kPer];
+        if (g.top != nullptr) {
+            const size_t o = static_cast<size_t>(t) * g.K + l;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const bool mine = there && l + i * kLanes < g.K;
+                const long long e = mine ? g.top[o + i * kLanes] : -1;
+                w[i] = mine ? g.weights[o + i * kLanes] : 0.0f;
+                dw[i] = mine ? g.d_weights[o + i * kLanes] : 0.0f;
+                expert[i] = e >= 0 && e < g.E ? static_cast<int>(e) : -1;
+            }
+        }
         bool live = there && losses && (g.mask == nullptr || g.mask[t]);
         if (g.offsets != nullptr && there) {
             while (s < g.S && seq_bound(g.offsets, s + 1, g.T) <= t) ++s;
@@ -547,55 +620,64 @@ __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceB
         }
         if (live && s != held) {
             load_row<V>(g.coef + static_cast<size_t>(s) * g.E, e0, g.E, g.coef_chunk, 0.0f, a);
+#pragma unroll
+            for (int j = 0; j < V; ++j) a[j] *= gb;
             held = s;
         }
-        float d[V], v[V];
-        const T* const row = static_cast<const T*>(g.logits) + static_cast<size_t>(there ? t : t0) * g.E;
-        if (losses) {
-            float p[V], q[V];
-            load_row<V>(row, e0, g.E, g.chunk, -INFINITY, v);
-            const float lse = row_probs<kLanes>(v, g.sigmoid, p, q);
+        if (kLanes == 32 ? live : losses) {            // shorter groups of a warp stay in step
+            float ex[V], sg[V];
+            const RowStats r = row_stats<kLanes, V, kSigmoid>(v, ex, sg);
             float dot = 0.0f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) dot += p[j] * a[j];
+            for (int j = 0; j < V; ++j) dot = fmaf(kSigmoid ? sg[j] : ex[j], a[j], dot);
             dot = group_sum<kLanes>(dot);
-            const float zs = gz * lse;
+            if constexpr (kSigmoid) {
+                dot *= r.inv_sg;
+                const float zs = gz * r.lse * r.inv;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float slope = p[j] * (a[j] - dot);
-                if (g.sigmoid) slope *= sigmoid_rest(v[j]);
-                d[j] = live ? gb * slope + zs * q[j] : 0.0f;
+                for (int j = 0; j < V; ++j) d[j] = fmaf(sg[j] * r.inv_sg * sigmoid_rest(v[j]), a[j] - dot, ex[j] * zs);
+            } else {
+                const float c = (gz * r.lse - dot * r.inv) * r.inv;
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[j] = ex[j] * fmaf(a[j], r.inv, c);
+            }
+            if constexpr (kLanes != 32) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[j] = live ? d[j] : 0.0f;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) d[j] = 0.0f;
         }
         if (g.top != nullptr) {
-            const size_t o = static_cast<size_t>(t) * g.K;
             float dot = 0.0f;
-            for (int k = l; k < g.K && there; k += kLanes) dot += g.weights[o + k] * g.d_weights[o + k];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) dot = fmaf(w[i], dw[i], dot);
             dot = group_sum<kLanes>(dot);
-            auto expert = [&](int k) { const long long e = g.top[o + k]; return e >= 0 && e < g.E ? static_cast<int>(e) : -1; };
-            auto value = [&](int k, int e) {
-                const float w = g.weights[o + k];
-                float x = w * (g.d_weights[o + k] - dot);
-                if (g.sigmoid) x *= sigmoid_rest(to_float(row[e]));
-                return w == 0.0f ? 0.0f : x;
-            };
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                dw[i] = w[i] == 0.0f ? 0.0f : w[i] * (dw[i] - dot);
+                if (kSigmoid && expert[i] >= 0) dw[i] *= sigmoid_rest(to_float(row[expert[i]]));
+                if (expert[i] >= 0) add[expert[i]] = __int_as_float(l + i * kLanes);
+            }
             // an expert that a row names twice (finished routes may) shows in the tag that was overwritten
             bool twice = false;
-            for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = __int_as_float(k); }
             __syncwarp();
-            for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); twice |= e >= 0 && __float_as_int(add[e]) != k; }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) twice |= expert[i] >= 0 && __float_as_int(add[expert[i]]) != l + i * kLanes;
             if (__any_sync(kAll, twice)) {
-                for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = 0.0f; }
-                for (int k = 0; k < g.K; ++k) {                   // one at a time, in order
-                    __syncwarp();
-                    if (there && k % kLanes == l) { const int e = expert(k); if (e >= 0) add[e] += value(k, e); }
-                }
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) if (expert[i] >= 0) add[expert[i]] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    for (int who = 0; who < kLanes; ++who) {       // one at a time, in order
+                        __syncwarp();
+                        if (l == who && expert[i] >= 0) add[expert[i]] += dw[i];
+                    }
             } else {
                 __syncwarp();
-                for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = value(k, e); }
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) if (expert[i] >= 0) add[expert[i]] = dw[i];
             }
             __syncwarp();
 #pragma unroll
@@ -604,7 +686,8 @@ __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceB
                 d[j] += x.x; d[j + 1] += x.y; d[j + 2] += x.z; d[j + 3] += x.w;
             }
             __syncwarp();
-            for (int k = l; k < g.K && there; k += kLanes) { const int e = expert(k); if (e >= 0) add[e] = 0.0f; }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) if (expert[i] >= 0) add[expert[i]] = 0.0f;
             __syncwarp();
         }
         if (there) store_row<V>(static_cast<T*>(g.d_logits) + static_cast<size_t>(t) * g.E, e0, g.E, g.chunk, d);
@@ -648,18 +731,19 @@ __global__ void __launch_bounds__(kRowThreads) expert_counts_kernel(const CountP
     }
 }
 
-template <typename T, int kLanes, int V>
+template <typename T, int kLanes, int V, bool kSigmoid>
 int launch_rows(const BalanceParams& p, cudaStream_t s) {
     const size_t chosen = p.top_in == nullptr ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
-    return launch_kernel(balance_rows_kernel<T, kLanes, V>, p.blocks, kRowThreads, (static_cast<size_t>(kWarps + 1) * p.E + chosen) * 4, s, false, true, p);
+    const size_t smem = (static_cast<size_t>(kWarps) * p.E + ((p.E + 1) & ~1) + chosen) * 4;
+    return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid>, p.blocks, kRowThreads, smem, s, false, true, p);
 }
 
-template <typename T, int kLanes, int V>
+template <typename T, int kLanes, int V, bool kSigmoid>
 int launch_bwd(BalanceBwdParams p, cudaStream_t s) {
     constexpr int kGroups = kRowThreads / kLanes;
     const int blocks = std::min((p.T + kGroups - 1) / kGroups, device_sm_count() * 8);
     p.rows_per_block = (p.T + blocks - 1) / blocks;
-    return launch_kernel(balance_bwd_kernel<T, kLanes, V>, blocks, kRowThreads, 0, s, false, true, p);
+    return launch_kernel(balance_bwd_kernel<T, kLanes, V, kSigmoid>, blocks, kRowThreads, 0, s, false, true, p);
 }
 
 // lanes a row and values a lane: four values where a row fits, so that 32 lanes hold several short rows
@@ -684,7 +768,7 @@ using namespace mok;
 
 extern "C" size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences) {
     if (bad_sizes(num_tokens, num_experts, 1, num_sequences)) return 0;
-    return Scratch(nullptr, row_blocks(num_tokens) + num_sequences, num_experts, num_sequences).bytes;
+    return Scratch(nullptr, row_blocks(num_tokens, num_experts) + num_sequences, num_experts, num_sequences).bytes;
 }
 
 extern "C" int mok_router_balance(const void* logits, int logits_bf16, int num_tokens, int num_experts, int topk, int num_sequences,
@@ -699,7 +783,7 @@ extern "C" int mok_router_balance(const void* logits, int logits_bf16, int num_t
     const int tiles = (num_experts + kJoinCols - 1) / kJoinCols;
     if (too_many_routes(num_tokens, topk) || static_cast<long long>(num_sequences) * tiles > 0x3fffffff) return MOK_ERR_TOO_LARGE;
     BalanceParams p{};
-    p.blocks = row_blocks(num_tokens);
+    p.blocks = row_blocks(num_tokens, num_experts);
     const Scratch at(scratch, p.blocks + num_sequences, num_experts, num_sequences);
     if (scratch_bytes < at.bytes || reinterpret_cast<uintptr_t>(scratch) % 16) return MOK_ERR_INVALID;
     p.logits = logits;
@@ -722,11 +806,11 @@ extern "C" int mok_router_balance(const void* logits, int logits_bf16, int num_t
     ProfScope prof(kSlotOther, s, 2);
     int rc;
     if (logits_bf16) {
-#define MOK_CALL(lanes, v) launch_rows<__nv_bfloat16, lanes, v>(p, s)
+#define MOK_CALL(lanes, v) (p.sigmoid ? launch_rows<__nv_bfloat16, lanes, v, true>(p, s) : launch_rows<__nv_bfloat16, lanes, v, false>(p, s))
         rc = MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
     } else {
-#define MOK_CALL(lanes, v) launch_rows<float, lanes, v>(p, s)
+#define MOK_CALL(lanes, v) (p.sigmoid ? launch_rows<float, lanes, v, true>(p, s) : launch_rows<float, lanes, v, false>(p, s))
         rc = MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
     }
@@ -742,7 +826,7 @@ extern "C" int mok_router_balance_bwd(const float* d_losses, const void* logits,
                                       int num_experts, int topk, int num_sequences, int sigmoid, void* stream) {
     if (!d_losses || !logits || !coef || !d_logits || bad_sizes(num_tokens, num_experts, topk, num_sequences)) return MOK_ERR_INVALID;
     const int with = (top_experts != nullptr) + (router_weights != nullptr) + (d_router_weights != nullptr);
-    if (with != 0 && (with != 3 || topk > 32)) return MOK_ERR_INVALID;
+    if (with != 0 && (with != 3 || topk > 32 || topk > num_experts)) return MOK_ERR_INVALID;
     if (!sequence_offsets && num_sequences != 1) return MOK_ERR_INVALID;
     if (num_experts > 1024) return MOK_ERR_UNSUPPORTED;
     BalanceBwdParams p{d_losses, logits, coef, token_mask, sequence_offsets, reinterpret_cast<const long long*>(top_experts),
@@ -752,11 +836,11 @@ extern "C" int mok_router_balance_bwd(const float* d_losses, const void* logits,
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(kSlotOther, s);
     if (logits_bf16) {
-#define MOK_CALL(lanes, v) launch_bwd<__nv_bfloat16, lanes, v>(p, s)
+#define MOK_CALL(lanes, v) (p.sigmoid ? launch_bwd<__nv_bfloat16, lanes, v, true>(p, s) : launch_bwd<__nv_bfloat16, lanes, v, false>(p, s))
         return MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
     }
-#define MOK_CALL(lanes, v) launch_bwd<float, lanes, v>(p, s)
+#define MOK_CALL(lanes, v) (p.sigmoid ? launch_bwd<float, lanes, v, true>(p, s) : launch_bwd<float, lanes, v, false>(p, s))
     return MOK_ROW_SHAPE(num_experts, MOK_CALL);
 #undef MOK_CALL
 }

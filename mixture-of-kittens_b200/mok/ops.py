@@ -1034,7 +1034,8 @@ def router_balance_bwd(d_losses: Tensor, logits: Tensor, coef: Tensor, token_mas
     _need(all(given) or not any(given), "top_experts, router_weights and d_router_weights come together or not at all")
     if all(given):
         T_routes, K = _routes(top_experts)
-        _need(T_routes == T and K <= 32 and top_experts.device == dev, "top_experts must be [num_tokens, topk <= 32] on the device of the logits")
+        _need(T_routes == T and K <= min(32, E) and top_experts.device == dev,
+              "top_experts must be [num_tokens, topk] with topk <= min(32, num_experts), on the device of the logits")
         for name, t in (("router_weights", router_weights), ("d_router_weights", d_router_weights)):
             _need(t.device == dev and tuple(t.shape) == (T, K) and t.is_contiguous(), f"{name} must be contiguous and match top_experts")
             _need(t.dtype == torch.float32, f"{name} must have dtype torch.float32", TypeError)

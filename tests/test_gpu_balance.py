@@ -250,6 +250,33 @@ def test_expert_counts(cuda_device, T, E, K, S, mask, dtype):
     assert got.dtype == torch.int32 and np.array_equal(got.cpu().numpy(), O.expert_counts(experts, E, **plain(where)))
 
 
+@pytest.mark.parametrize("T,E,K", [(7, 5, 4), (130, 30, 17), (90, 64, 32), (33, 128, 9), (50, 700, 32)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_weight_gradients_of_an_expert_named_twice_add_up(cuda_device, T, E, K, sigmoid):
+    """And ids outside [0, E) get none.  Bound: K additions and the terms' own roundings, 240 u of their magnitude."""
+    from mok import ops
+    rng = np.random.default_rng(K)
+    experts = rng.integers(-1, max(2, E // 3), (T, K))
+    logits = rng.standard_normal((T, E)).astype(np.float32)
+    w, dw = rng.random((T, K)).astype(np.float32), rng.standard_normal((T, K)).astype(np.float32)
+    w[0, 0] = 0.0
+    d = lambda a: torch.from_numpy(a).to(cuda_device)                                    # noqa: E731
+    args = (torch.zeros(2, device=cuda_device), d(logits), torch.zeros(E + 2, device=cuda_device), None, None, d(experts), d(w), d(dw), sigmoid)
+    got = ops.router_balance_bwd(*args)
+    assert torch.equal(got, ops.router_balance_bwd(*args))
+    term = w.astype(np.float64) * (dw - (w.astype(np.float64) * dw).sum(1, keepdims=True))
+    size = w.astype(np.float64) * (np.abs(dw) + np.abs(w.astype(np.float64) * dw).sum(1, keepdims=True))
+    want, scale = np.zeros((T, E)), np.zeros((T, E))
+    for t in range(T):
+        for k in range(K):
+            e = experts[t, k]
+            if e >= 0:
+                f = 1 / (1 + np.exp(float(logits[t, e]))) if sigmoid else 1.0
+                want[t, e] += term[t, k] * f
+                scale[t, e] += size[t, k] * f
+    assert (np.abs(got.cpu().numpy() - want) <= GRAD * scale).all()
+
+
 def test_no_tokens(cuda_device):
     from mok import functional as F, ops
     logits = torch.zeros(0, 8, device=cuda_device)
@@ -288,7 +315,7 @@ def test_refusals(cuda_device):
     g, coef = torch.ones(2, device=cuda_device), torch.ones(8, device=cuda_device)
     w = torch.ones(8, 2, device=cuda_device)
     for args in ((g[:1], x, coef), (g, x, coef[:7]), (g, x, coef, None, i32(3)), (g, x, coef, None, None, ids, w),
-                 (g, x, coef, None, None, ids, w, w[:, :1]), (g, x, coef, None, None, ids[:4], w, w), (g.cpu(), x, coef)):
+                 (g, x, coef, None, None, ids.repeat(1, 4), w.repeat(1, 4), w.repeat(1, 4)), (g, x, coef, None, None, ids, w, w[:, :1]), (g, x, coef, None, None, ids[:4], w, w), (g.cpu(), x, coef)):
         with pytest.raises(ValueError):
             ops.router_balance_bwd(*args)
     with pytest.raises(TypeError):

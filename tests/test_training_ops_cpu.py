@@ -121,7 +121,7 @@ def test_c_entries_refuse_bad_arguments():
     assert L.mok_router_balance_scratch_bytes(0, 8, 1) == 0
     bwd = lambda *, g=p, T=512, E=8, K=2, S=1, top=z, w=z, dw=z, off=z: L.mok_router_balance_bwd(                              # noqa: E731
         g, p, 0, p, z, off, top, w, dw, p, T, E, K, S, 0, z)
-    assert bwd(g=z) == bwd(T=0) == bwd(S=3) == bwd(top=p) == bwd(top=p, w=p) == bwd(top=p, w=p, dw=p, K=33) == -1
+    assert bwd(g=z) == bwd(T=0) == bwd(S=3) == bwd(top=p) == bwd(top=p, w=p) == bwd(top=p, w=p, dw=p, K=33, E=64) == bwd(top=p, w=p, dw=p, K=9) == -1
     assert bwd(E=2000) == -3
     counts = lambda *, ids=p, T=512, E=8, K=2, S=1, off=z: L.mok_expert_counts(ids, 0, T, K, E, S, z, off, p, z)              # noqa: E731
     assert counts(ids=z) == counts(T=-1) == counts(E=0) == counts(S=2) == -1
