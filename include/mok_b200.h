@@ -175,15 +175,36 @@ int mok_router_topk_bwd(const int32_t* top_experts_i32, const float* router_weig
  * mok_router_balance_bwd writes all of d_logits (type of logits) from d_losses f32 [2] and, where the three are not NULL,
  * from the gradient of the router weights (topk <= 32 and <= num_experts).
  * No reference counterpart (the reference takes finished routes and returns no losses). */
+typedef struct mok_router_balance_args {
+    const void* logits;
+    const int64_t* top_experts_in;
+    int64_t* top_experts_out;
+    float* router_weights;
+    const uint8_t* token_mask;
+    const int32_t* sequence_offsets;
+    const int32_t* load;
+    float* losses;
+    int32_t* counts;
+    float* coef;
+    void* scratch;
+    size_t scratch_bytes;
+    int logits_bf16, num_tokens, num_experts, topk, num_sequences, sigmoid;
+} mok_router_balance_args;
+typedef struct mok_router_balance_bwd_args {
+    const float* d_losses;
+    const void* logits;
+    const float* coef;
+    const uint8_t* token_mask;
+    const int32_t* sequence_offsets;
+    const int64_t* top_experts;
+    const float* router_weights;
+    const float* d_router_weights;
+    void* d_logits;
+    int logits_bf16, num_tokens, num_experts, topk, num_sequences, sigmoid;
+} mok_router_balance_bwd_args;
 size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences);
-int mok_router_balance(const void* logits, int logits_bf16, int num_tokens, int num_experts, int topk, int num_sequences,
-                       int sigmoid, const int64_t* top_experts_in, int64_t* top_experts_out, float* router_weights,
-                       const uint8_t* token_mask, const int32_t* sequence_offsets, const int32_t* load, float* losses,
-                       int32_t* counts, float* coef, void* scratch, size_t scratch_bytes, void* stream);
-int mok_router_balance_bwd(const float* d_losses, const void* logits, int logits_bf16, const float* coef,
-                           const uint8_t* token_mask, const int32_t* sequence_offsets, const int64_t* top_experts,
-                           const float* router_weights, const float* d_router_weights, void* d_logits, int num_tokens,
-                           int num_experts, int topk, int num_sequences, int sigmoid, void* stream);
+int mok_router_balance(const mok_router_balance_args* args, void* stream);
+int mok_router_balance_bwd(const mok_router_balance_bwd_args* args, void* stream);
 
 /* counts int32 [num_sequences, num_experts] of routes [num_tokens, topk] (int64, or int32 with ids_i32 != 0; ids outside
  * [0, num_experts) are not counted), of the rows that count as above.  No reference counterpart. */

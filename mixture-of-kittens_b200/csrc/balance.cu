@@ -58,7 +58,10 @@ struct Scratch {
     }
 };
 
-int row_blocks(int T, int E) { return std::min(148 * row_blocks_per_sm(E), (T + kWarps - 1) / kWarps); }
+int row_blocks(int T, int E) {
+    const int rows = kWarps * (E <= 16 ? 8 : E <= 32 ? 4 : E <= 64 ? 2 : 1);                 // that a block works on at once
+    return std::min(148 * row_blocks_per_sm(E), (T + rows - 1) / rows);
+}
 
 // how rows of E values of `bytes` bytes at `base` can be read: chunks of eight (16 or 32 bytes), of four, or one by one
 int chunk_of(const void* base, int E, int bytes) {
@@ -315,48 +318,76 @@ __device__ __forceinline__ void select_in_rounds(const float (&v)[V], int E, int
     __syncwarp();
 }
 
-// One row a warp: with t the K-th largest of the lanes' maxima, at least K values are >= t and only few more; they are
-// gathered, one a lane, and every lane counts those that come before its own.  Rows where that does not work out (fewer than K
-// lanes with a value above -inf, more than 32 values >= t) go in rounds.  131072 rows of 256, K = 8, rounds -> this, forward:
-// see the figures at balance_rows_kernel.
+__device__ __forceinline__ float warp_min(float v) {
+    float m;
+    asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+
+// Values >= t into gathered[0..min(n, 32)), one slot each in no order that matters; returns how many there are.
 template <int V>
-__device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K, float2* gathered, float2* chosen) {
+__device__ __forceinline__ int gather_above(const float (&v)[V], float t, uint2* gathered) {
+    const int lane = threadIdx.x & 31;
+    const unsigned below = (1u << lane) - 1u;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const bool in = v[j] >= t;
+        const unsigned at = __ballot_sync(kAll, in);
+        if (V <= 8 || at != 0) {
+            if (in) gathered[(n + __popc(at & below)) & 31] = make_uint2(lane * V + j, __float_as_uint(v[j]));
+            n += __popc(at);
+        }
+    }
+    return n;
+}
+
+// One row a warp.  Let the lanes form at least K sets of `set` neighbours, and t be the least of the sets' maxima: at least K
+// values are >= t, and few more.  They are gathered, one a lane, and every lane counts those that come before its own.  Where
+// more than 32 are >= t (with K = 8 of 256 in few rows of a hundred), t is the K-th largest of the lanes' maxima instead, and
+// where that does not do either (many equal values, few above -inf, no such sets: set = 0) the row goes in rounds.
+template <int V>
+__device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K, int set, uint2* gathered, float2* chosen) {
     const int lane = threadIdx.x & 31;
     float b = v[0];
 #pragma unroll
     for (int j = 1; j < V; ++j) b = fmaxf(b, v[j]);
     b = b > -INFINITY ? b : -INFINITY;                             // all NaN
-    float t;
-    int found = 0;
-    do {
-        t = group_max<32>(b);
-        const bool equal = b == t;
-        found += __popc(__ballot_sync(kAll, equal));
-        b = equal ? -INFINITY : b;
-    } while (found < K && t > -INFINITY);
-    int n = 0;
-    if (t > -INFINITY) {
-        const unsigned below = (1u << lane) - 1u;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const bool in = v[j] >= t;
-            const unsigned at = __ballot_sync(kAll, in);
-            const int to = n + __popc(at & below);
-            if (in && to < 32) gathered[to] = make_float2(v[j], __int_as_float(lane * V + j));
-            n += __popc(at);
-        }
+    float t = b;
+    if (set >= 2) t = fmaxf(t, __shfl_xor_sync(kAll, t, 1));
+    if (set >= 4) t = fmaxf(t, __shfl_xor_sync(kAll, t, 2));
+    t = warp_min(((lane | (set - 1)) + 1) * V <= E ? t : INFINITY);           // sets of lanes that are full
+    int n = 33;
+    if (set > 0 && t > -INFINITY) n = gather_above(v, t, gathered);
+    if (n > 32) {
+        int found = 0;
+        do {
+            t = group_max<32>(b);
+            const bool equal = b == t;
+            found += __popc(__ballot_sync(kAll, equal));
+            b = equal ? -INFINITY : b;
+        } while (found < K && t > -INFINITY);
+        __syncwarp();
+        if (t > -INFINITY) n = gather_above(v, t, gathered);
+        if (n > 32) { select_in_rounds<32, V>(v, E, K, chosen); return; }
     }
-    if (t == -INFINITY || n > 32) { select_in_rounds<32, V>(v, E, K, chosen); return; }
     __syncwarp();
-    const float2 mine = gathered[lane];                            // past n: left over, not used
-    const int e = __float_as_int(mine.y);
+    // (value, expert) as one 64-bit number that grows with the value (-0 as 0) and falls with the expert
+    const uint2 own = gathered[lane];                              // past n: left over, not used
+    const float value = __uint_as_float(own.y) + 0.0f;
+    const unsigned bits = __float_as_uint(value);
+    const unsigned order = bits ^ (static_cast<int>(bits) < 0 ? 0xffffffffu : 0x80000000u);
+    unsigned long long* const keys = reinterpret_cast<unsigned long long*>(gathered);
+    const unsigned long long key = lane < n ? static_cast<unsigned long long>(order) << 32 | (0xffffffffu - own.x) : 0ull;
+    keys[lane] = key;
+    __syncwarp();
     int before = 0;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float2 other = gathered[i];
-        before += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
+#pragma unroll 2
+    for (int i = 0; i < n; i += 4) {                               // past n: 0, before nothing
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(keys + i), c = *reinterpret_cast<const ulonglong2*>(keys + i + 2);
+        before += (a.x > key) + (a.y > key) + (c.x > key) + (c.y > key);
     }
-    if (lane < n && before < K) chosen[before] = mine;
+    if (lane < n && before < K) chosen[before] = make_float2(__uint_as_float(own.y), __int_as_float(static_cast<int>(own.x)));
     __syncwarp();
 }
 
@@ -364,8 +395,9 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
 template <typename T, int kLanes, int V, bool kSigmoid>
 __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) balance_rows_kernel(const BalanceParams g) {
     constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
+    constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // chosen experts a lane, at most (K <= 32 and <= E)
     extern __shared__ float smem[];                            // p [kWarps][E], routes [E], then the chosen (value, expert) [kGroups][K]
-    __shared__ float2 s_gathered[kWarps][32];
+    __shared__ alignas(16) uint2 s_gathered[kLanes == 32 ? kWarps : 1][32];
     __shared__ float s_z[kWarps];
     __shared__ int s_rows[kWarps], s_routes;
     int* const hist = reinterpret_cast<int*>(smem + static_cast<size_t>(kWarps) * g.E);
@@ -375,6 +407,8 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
     const bool select = g.top_in == nullptr;
+    const int full = g.E / V;                                  // lanes that hold V values (select_by_rank: sets of 4, 2 or 1 of them)
+    const int set = full / 4 >= g.K ? 4 : full / 2 >= g.K ? 2 : full >= g.K ? 1 : 0;
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
@@ -413,22 +447,31 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
                 }
             }
             if (select) {
-                if constexpr (kLanes == 32) select_by_rank<V>(v, g.E, g.K, s_gathered[warp], chosen);
+                if constexpr (kLanes == 32) select_by_rank<V>(v, g.E, g.K, set, s_gathered[warp], chosen);
                 else select_in_rounds<kLanes, V>(v, g.E, g.K, chosen);
                 const float top = chosen[0].x;
                 auto weight = [&](float x) {
                     return top == -INFINITY ? 0.0f : kSigmoid ? sigmoid_scaled(x, top) : exp2_fast((x - top) * kLog2e);
                 };
-                float sum = 0.0f;
-                for (int k = l; k < g.K; k += kLanes) sum += weight(chosen[k].x);
+                float w[kPer], sum = 0.0f;
+                int e[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const bool mine = l + i * kLanes < g.K;
+                    const float2 c = mine ? chosen[l + i * kLanes] : make_float2(0.0f, 0.0f);
+                    e[i] = __float_as_int(c.y);
+                    w[i] = mine ? weight(c.x) : 0.0f;
+                    sum += w[i];
+                }
                 sum = group_sum<kLanes>(sum);
                 const float inv = sum == 0.0f ? 0.0f : rcp_fast(sum);
-                for (int k = l; k < g.K && there; k += kLanes) {
-                    const float2 c = chosen[k];
-                    const int e = __float_as_int(c.y);
-                    g.top_out[o + k] = e;
-                    g.weights[o + k] = weight(c.x) * inv;
-                    if (live) { atomicAdd(&hist[e], 1); ++routes; }
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    if (there && l + i * kLanes < g.K) {
+                        g.top_out[o + l + i * kLanes] = e[i];
+                        g.weights[o + l + i * kLanes] = w[i] * inv;
+                        if (live) { atomicAdd(&hist[e[i]], 1); ++routes; }
+                    }
                 }
                 __syncwarp();
             } else if (live) {
@@ -771,77 +814,77 @@ extern "C" size_t mok_router_balance_scratch_bytes(int num_tokens, int num_exper
     return Scratch(nullptr, row_blocks(num_tokens, num_experts) + num_sequences, num_experts, num_sequences).bytes;
 }
 
-extern "C" int mok_router_balance(const void* logits, int logits_bf16, int num_tokens, int num_experts, int topk, int num_sequences,
-                                  int sigmoid, const int64_t* top_experts_in, int64_t* top_experts_out, float* router_weights,
-                                  const uint8_t* token_mask, const int32_t* sequence_offsets, const int32_t* load, float* losses,
-                                  int32_t* counts, float* coef, void* scratch, size_t scratch_bytes, void* stream) {
-    if (!logits || !losses || !counts || !coef || !scratch || bad_sizes(num_tokens, num_experts, topk, num_sequences)) return MOK_ERR_INVALID;
-    if ((top_experts_in == nullptr) != (top_experts_out != nullptr && router_weights != nullptr)) return MOK_ERR_INVALID;
-    if (!top_experts_in && (topk > 32 || topk > num_experts)) return MOK_ERR_INVALID;
-    if (!sequence_offsets && num_sequences != 1) return MOK_ERR_INVALID;
-    if (num_experts > 1024) return MOK_ERR_UNSUPPORTED;
-    const int tiles = (num_experts + kJoinCols - 1) / kJoinCols;
-    if (too_many_routes(num_tokens, topk) || static_cast<long long>(num_sequences) * tiles > 0x3fffffff) return MOK_ERR_TOO_LARGE;
+extern "C" int mok_router_balance(const mok_router_balance_args* args, void* stream) {
+    if (!args) return MOK_ERR_INVALID;
+    const mok_router_balance_args& a = *args;
+    const int T = a.num_tokens, E = a.num_experts, K = a.topk, S = a.num_sequences;
+    if (!a.logits || !a.losses || !a.counts || !a.coef || !a.scratch || bad_sizes(T, E, K, S)) return MOK_ERR_INVALID;
+    if (a.top_experts_in ? (a.top_experts_out || a.router_weights) : (!a.top_experts_out || !a.router_weights)) return MOK_ERR_INVALID;
+    if (!a.top_experts_in && (K > 32 || K > E)) return MOK_ERR_INVALID;
+    if (!a.sequence_offsets && S != 1) return MOK_ERR_INVALID;
+    if (E > 1024) return MOK_ERR_UNSUPPORTED;
+    const int tiles = (E + kJoinCols - 1) / kJoinCols;
+    if (too_many_routes(T, K) || static_cast<long long>(S) * tiles > 0x3fffffff) return MOK_ERR_TOO_LARGE;
     BalanceParams p{};
-    p.blocks = row_blocks(num_tokens, num_experts);
-    const Scratch at(scratch, p.blocks + num_sequences, num_experts, num_sequences);
-    if (scratch_bytes < at.bytes || reinterpret_cast<uintptr_t>(scratch) % 16) return MOK_ERR_INVALID;
-    p.logits = logits;
-    p.top_in = reinterpret_cast<const long long*>(top_experts_in);
-    p.top_out = reinterpret_cast<long long*>(top_experts_out);
-    p.weights = router_weights;
-    p.mask = token_mask;
-    p.offsets = sequence_offsets;
-    p.load = load;
-    p.losses = losses;
-    p.counts = counts;
-    p.coef = coef;
-    p.T = num_tokens; p.E = num_experts; p.K = topk; p.S = num_sequences;
-    p.rows_per_block = (num_tokens + p.blocks - 1) / p.blocks;
-    p.sigmoid = sigmoid;
-    p.chunk = chunk_of(logits, num_experts, logits_bf16 ? 2 : 4);
+    p.blocks = row_blocks(T, E);
+    const Scratch at(a.scratch, p.blocks + S, E, S);
+    if (a.scratch_bytes < at.bytes || reinterpret_cast<uintptr_t>(a.scratch) % 16) return MOK_ERR_INVALID;
+    p.logits = a.logits;
+    p.top_in = reinterpret_cast<const long long*>(a.top_experts_in);
+    p.top_out = reinterpret_cast<long long*>(a.top_experts_out);
+    p.weights = a.router_weights;
+    p.mask = a.token_mask;
+    p.offsets = a.sequence_offsets;
+    p.load = a.load;
+    p.losses = a.losses;
+    p.counts = a.counts;
+    p.coef = a.coef;
+    p.T = T; p.E = E; p.K = K; p.S = S;
+    p.rows_per_block = (T + p.blocks - 1) / p.blocks;
+    p.sigmoid = a.sigmoid;
+    p.chunk = chunk_of(a.logits, E, a.logits_bf16 ? 2 : 4);
     p.head = at.head; p.slot_p = at.p; p.slot_routes = at.routes; p.part = at.part; p.seq_z = at.seq_z; p.seq_rows = at.seq_rows;
     p.ticket = at.ticket;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(kSlotOther, s, 2);
     int rc;
-    if (logits_bf16) {
+    if (a.logits_bf16) {
 #define MOK_CALL(lanes, v) (p.sigmoid ? launch_rows<__nv_bfloat16, lanes, v, true>(p, s) : launch_rows<__nv_bfloat16, lanes, v, false>(p, s))
-        rc = MOK_ROW_SHAPE(num_experts, MOK_CALL);
+        rc = MOK_ROW_SHAPE(E, MOK_CALL);
 #undef MOK_CALL
     } else {
 #define MOK_CALL(lanes, v) (p.sigmoid ? launch_rows<float, lanes, v, true>(p, s) : launch_rows<float, lanes, v, false>(p, s))
-        rc = MOK_ROW_SHAPE(num_experts, MOK_CALL);
+        rc = MOK_ROW_SHAPE(E, MOK_CALL);
 #undef MOK_CALL
     }
     if (rc != MOK_OK) return rc;
     // warps for the slots of a sequence, on average
-    if (p.blocks / num_sequences >= 64) return launch_kernel(balance_join_kernel<32>, num_sequences * tiles, 1024, 0, s, false, true, p);
-    return launch_kernel(balance_join_kernel<8>, num_sequences * tiles, 256, 0, s, false, true, p);
+    if (p.blocks / S >= 64) return launch_kernel(balance_join_kernel<32>, S * tiles, 1024, 0, s, false, true, p);
+    return launch_kernel(balance_join_kernel<8>, S * tiles, 256, 0, s, false, true, p);
 }
 
-extern "C" int mok_router_balance_bwd(const float* d_losses, const void* logits, int logits_bf16, const float* coef,
-                                      const uint8_t* token_mask, const int32_t* sequence_offsets, const int64_t* top_experts,
-                                      const float* router_weights, const float* d_router_weights, void* d_logits, int num_tokens,
-                                      int num_experts, int topk, int num_sequences, int sigmoid, void* stream) {
-    if (!d_losses || !logits || !coef || !d_logits || bad_sizes(num_tokens, num_experts, topk, num_sequences)) return MOK_ERR_INVALID;
-    const int with = (top_experts != nullptr) + (router_weights != nullptr) + (d_router_weights != nullptr);
-    if (with != 0 && (with != 3 || topk > 32 || topk > num_experts)) return MOK_ERR_INVALID;
-    if (!sequence_offsets && num_sequences != 1) return MOK_ERR_INVALID;
-    if (num_experts > 1024) return MOK_ERR_UNSUPPORTED;
-    BalanceBwdParams p{d_losses, logits, coef, token_mask, sequence_offsets, reinterpret_cast<const long long*>(top_experts),
-                       router_weights, d_router_weights, d_logits, num_tokens, num_experts, topk, num_sequences, sigmoid, 0,
-                       std::min(chunk_of(logits, num_experts, logits_bf16 ? 2 : 4), chunk_of(d_logits, num_experts, logits_bf16 ? 2 : 4)),
-                       chunk_of(coef, num_experts, 4)};
+extern "C" int mok_router_balance_bwd(const mok_router_balance_bwd_args* args, void* stream) {
+    if (!args) return MOK_ERR_INVALID;
+    const mok_router_balance_bwd_args& a = *args;
+    const int T = a.num_tokens, E = a.num_experts, K = a.topk, S = a.num_sequences, bytes = a.logits_bf16 ? 2 : 4;
+    if (!a.d_losses || !a.logits || !a.coef || !a.d_logits || bad_sizes(T, E, K, S)) return MOK_ERR_INVALID;
+    const int with = (a.top_experts != nullptr) + (a.router_weights != nullptr) + (a.d_router_weights != nullptr);
+    if (with != 0 && (with != 3 || K > 32 || K > E)) return MOK_ERR_INVALID;
+    if (!a.sequence_offsets && S != 1) return MOK_ERR_INVALID;
+    if (E > 1024) return MOK_ERR_UNSUPPORTED;
+    if (static_cast<long long>(S) * E > 0x7fffffffll) return MOK_ERR_TOO_LARGE;
+    BalanceBwdParams p{a.d_losses, a.logits, a.coef, a.token_mask, a.sequence_offsets, reinterpret_cast<const long long*>(a.top_experts),
+                       a.router_weights, a.d_router_weights, a.d_logits, T, E, K, S, a.sigmoid, 0,
+                       std::min(chunk_of(a.logits, E, bytes), chunk_of(a.d_logits, E, bytes)), chunk_of(a.coef, E, 4)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(kSlotOther, s);
-    if (logits_bf16) {
+    if (a.logits_bf16) {
 #define MOK_CALL(lanes, v) (p.sigmoid ? launch_bwd<__nv_bfloat16, lanes, v, true>(p, s) : launch_bwd<__nv_bfloat16, lanes, v, false>(p, s))
-        return MOK_ROW_SHAPE(num_experts, MOK_CALL);
+        return MOK_ROW_SHAPE(E, MOK_CALL);
 #undef MOK_CALL
     }
 #define MOK_CALL(lanes, v) (p.sigmoid ? launch_bwd<float, lanes, v, true>(p, s) : launch_bwd<float, lanes, v, false>(p, s))
-    return MOK_ROW_SHAPE(num_experts, MOK_CALL);
+    return MOK_ROW_SHAPE(E, MOK_CALL);
 #undef MOK_CALL
 }
 

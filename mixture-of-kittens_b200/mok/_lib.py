@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -136,10 +137,11 @@ mok_bwd_epilogue = _sig("mok_bwd_epilogue", C.c_int, [vp, vp, vp, C.c_int, C.c_i
 mok_router_topk = _sig("mok_router_topk", C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, vp, vp, u64p, C.c_int, C.c_int, vp])
 mok_router_topk_bwd = _sig("mok_router_topk_bwd", C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp])
 mok_router_balance_scratch_bytes = _sig("mok_router_balance_scratch_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int])
-mok_router_balance = _sig("mok_router_balance", C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp,
-                                                          vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp])
-mok_router_balance_bwd = _sig("mok_router_balance_bwd", C.c_int, [vp, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp, C.c_int, C.c_int,
-                                                                  C.c_int, C.c_int, C.c_int, vp])
+# the argument structs of these two as bytes: packing them costs a third of passing that many arguments
+pack_router_balance = struct.Struct("11PN6i").pack
+pack_router_balance_bwd = struct.Struct("9P6i").pack
+mok_router_balance = _sig("mok_router_balance", C.c_int, [C.c_char_p, vp])
+mok_router_balance_bwd = _sig("mok_router_balance_bwd", C.c_int, [C.c_char_p, vp])
 mok_expert_counts = _sig("mok_expert_counts", C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp])
 mok_dropout_add = _sig("mok_dropout_add", C.c_int, [vp, vp, vp, vp, C.c_int64, C.c_int, C.c_double, vp])
 mok_fwd_epilogue_rows = _sig("mok_fwd_epilogue_rows", C.c_int,

@@ -11,6 +11,7 @@ Deliberate differences from the reference:
 """
 from __future__ import annotations
 
+import functools
 import inspect
 import operator
 
@@ -78,9 +79,10 @@ class _EagerOp(torch.library.CustomOpDef):
                 or _forward_ad._current_level >= 0 or not _registered.isdisjoint(self.mok_other_kernels)):
             return False
         types = tuple(map(type, args))
-        if types not in self.mok_accepted and not self._accepts(types):
+        pick = self.mok_accepted.get(types) or self._accepts(types)
+        if pick is None:
             return False
-        tensors = self.mok_tensors(args)
+        tensors = pick(args)
         if _grad_enabled() and any(map(_requires_grad, tensors)):
             return False
         try:
@@ -88,13 +90,16 @@ class _EagerOp(torch.library.CustomOpDef):
         except RuntimeError:                                    # sparse and the like: no memory to point to
             return False
 
-    def _accepts(self, types) -> bool:
+    def _accepts(self, types):
+        """What picks the tensors of a call with arguments of these types, or None: not for the short way."""
         if not (self.mok_required <= len(types) <= len(self.mok_types)
                 and all(t in exact for t, exact in zip(types, self.mok_types))):
-            return False
-        if len(self.mok_accepted) < 64:                         # tensors and parameters mix in a few ways
-            self.mok_accepted.add(types)
-        return True
+            return None
+        at = [i for i, (t, exact) in enumerate(zip(types, self.mok_types)) if Tensor in exact and t is not type(None)]
+        pick = operator.itemgetter(*at) if len(at) > 1 else lambda args: (args[at[0]],)
+        if len(self.mok_accepted) < 64:                         # tensors, parameters and omitted tensors mix in a few ways
+            self.mok_accepted[types] = pick
+        return pick
 
 
 def _operator(name: str, mutates_args, schema: str | None = None):
@@ -106,12 +111,7 @@ def _operator(name: str, mutates_args, schema: str | None = None):
         params = list(inspect.signature(body).parameters.values())
         op.mok_body = body
         op.mok_types = tuple(_EXACT[p.annotation] for p in params)
-        op.mok_accepted = set()
-        at = [i for i, exact in enumerate(op.mok_types) if exact[0] is Tensor]
-        if any(type(None) in exact and Tensor in exact for exact in op.mok_types):
-            op.mok_tensors = lambda args: [args[i] for i in at if i < len(args) and args[i] is not None]
-        else:
-            op.mok_tensors = operator.itemgetter(*at) if len(at) > 1 else lambda args: (args[at[0]],)
+        op.mok_accepted = {}
         op.mok_required = sum(p.default is inspect.Parameter.empty for p in params)
         op.mok_mutated = tuple(i for i, p in enumerate(params) if p.name in mutates_args)
         op.mok_other_kernels = frozenset("/".join(name.split("::") + [key]) for key in _KERNEL_KEYS) - torch.library._impls
@@ -931,57 +931,67 @@ torch.library.register_autograd("mok::router_topk", _router_backward, setup_cont
 # ------------------------------------------------------------------------------------------
 # losses that keep the experts evenly used, and the counts behind them (no reference op)
 # ------------------------------------------------------------------------------------------
+_F32, _BF16, _I32, _I64, _BOOL = torch.float32, torch.bfloat16, torch.int32, torch.int64, torch.bool
+
+
 def _sequences(T: int, device, token_mask: Tensor | None, sequence_offsets: Tensor | None) -> int:
     """Checks the two ways of saying which tokens count; returns the number of sequences."""
-    if token_mask is not None:
-        _need(token_mask.device == device and token_mask.dtype == torch.bool and token_mask.is_contiguous()
-              and tuple(token_mask.shape) == (T,), "token_mask must be a contiguous bool tensor [num_tokens] on the device of the logits "
-              "or routes")
+    if token_mask is not None and not (token_mask.dtype is _BOOL and token_mask.shape == (T,) and token_mask.is_contiguous()
+                                       and token_mask.device == device):
+        raise ValueError("token_mask must be a contiguous bool tensor [num_tokens] on the device of the logits or routes")
     if sequence_offsets is None:
         return 1
-    _need(sequence_offsets.device == device and sequence_offsets.dtype == torch.int32 and sequence_offsets.is_contiguous()
-          and sequence_offsets.ndim == 1 and sequence_offsets.numel() >= 2,
-          "sequence_offsets must be a contiguous int32 tensor [num_sequences + 1] on the device of the logits or routes")
+    if not (sequence_offsets.dtype is _I32 and sequence_offsets.ndim == 1 and sequence_offsets.numel() >= 2
+            and sequence_offsets.is_contiguous() and sequence_offsets.device == device):
+        raise ValueError("sequence_offsets must be a contiguous int32 tensor [num_sequences + 1] on the device of the logits or routes")
     return sequence_offsets.numel() - 1
 
 
 def _balance_logits(logits: Tensor) -> tuple[int, int]:
-    _need(logits.is_cuda and logits.ndim == 2 and logits.is_contiguous(),
-          "logits must be a contiguous CUDA tensor of shape (num_tokens, num_experts)")
-    _need(logits.dtype in (torch.float32, torch.bfloat16), "logits must have dtype torch.float32 or torch.bfloat16", TypeError)
+    if not (logits.is_cuda and logits.ndim == 2 and logits.is_contiguous()):
+        raise ValueError("logits must be a contiguous CUDA tensor of shape (num_tokens, num_experts)")
+    if logits.dtype is not _F32 and logits.dtype is not _BF16:
+        raise TypeError("logits must have dtype torch.float32 or torch.bfloat16")
     T, E = logits.shape
-    _need(0 < E <= 1024, "num_experts must be in [1, 1024]")
+    if not 0 < E <= 1024:
+        raise ValueError("num_experts must be in [1, 1024]")
     return T, E
 
 
-def _routes(top_experts: Tensor, dtypes=(torch.int64,)) -> tuple[int, int]:
-    _need(top_experts.is_cuda and top_experts.ndim == 2 and top_experts.is_contiguous(),
-          "top_experts must be a contiguous CUDA tensor of shape (num_tokens, topk)")
-    _need(top_experts.dtype in dtypes, f"top_experts must have dtype {' or '.join(map(str, dtypes))}", TypeError)
+def _routes(top_experts: Tensor, dtypes=(_I64,)) -> tuple[int, int]:
+    if not (top_experts.is_cuda and top_experts.ndim == 2 and top_experts.is_contiguous()):
+        raise ValueError("top_experts must be a contiguous CUDA tensor of shape (num_tokens, topk)")
+    if top_experts.dtype not in dtypes:
+        raise TypeError(f"top_experts must have dtype {' or '.join(map(str, dtypes))}")
     T, K = top_experts.shape
-    _need(0 < K <= 255, "topk must be in [1, 255]")
+    if not 0 < K <= 255:
+        raise ValueError("topk must be in [1, 255]")
     return T, K
 
 
-def _run_balance(logits: Tensor, K: int, top_in: Tensor | None, experts: Tensor | None, weights: Tensor | None,
-                 token_mask: Tensor | None, sequence_offsets: Tensor | None, load: Tensor | None, sigmoid: bool, what: str):
-    T, E = logits.shape
+_balance_scratch_bytes = functools.lru_cache(maxsize=256)(_lib.mok_router_balance_scratch_bytes)     # a function of its arguments
+
+
+def _run_balance(logits: Tensor, T: int, E: int, K: int, top_in: int, experts: int, weights: int, token_mask: Tensor | None,
+                 sequence_offsets: Tensor | None, load: Tensor | None, sigmoid: bool, what: str):
     dev = logits.device
-    S = _sequences(T, dev, token_mask, sequence_offsets)
-    if load is not None:
-        _need(load.device == dev and load.dtype == torch.int32 and load.is_contiguous() and tuple(load.shape) == (S, E),
-              "load must be a contiguous int32 tensor (num_sequences, num_experts) on the device of the logits")
-    _need(type(sigmoid) is bool, "sigmoid must be a boolean", TypeError)
-    make = torch.empty if T > 0 else torch.zeros
-    losses = make(2, dtype=torch.float32, device=dev)
-    counts = make(S, E, dtype=torch.int32, device=dev)
-    coef = make(S * E + 2, dtype=torch.float32, device=dev)
-    if T > 0:
-        nbytes = _lib.mok_router_balance_scratch_bytes(T, E, S)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.launch(dev, what, _lib.mok_router_balance, logits.data_ptr(), logits.dtype == torch.bfloat16, T, E, K, S, sigmoid,
-                    _vp(top_in), _vp(experts), _vp(weights), _vp(token_mask), _vp(sequence_offsets), _vp(load), losses.data_ptr(),
-                    counts.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes)
+    S = 1 if token_mask is None and sequence_offsets is None else _sequences(T, dev, token_mask, sequence_offsets)
+    if load is not None and not (load.dtype is _I32 and load.shape == (S, E) and load.is_contiguous() and load.device == dev):
+        raise ValueError("load must be a contiguous int32 tensor (num_sequences, num_experts) on the device of the logits")
+    if type(sigmoid) is not bool:
+        raise TypeError("sigmoid must be a boolean")
+    if T == 0:
+        return (torch.zeros(2, dtype=_F32, device=dev), torch.zeros(S, E, dtype=_I32, device=dev),
+                torch.zeros(S * E + 2, dtype=_F32, device=dev))
+    losses = torch.empty(2, dtype=_F32, device=dev)
+    counts = torch.empty(S, E, dtype=_I32, device=dev)
+    coef = torch.empty(S * E + 2, dtype=_F32, device=dev)
+    nbytes = _balance_scratch_bytes(T, E, S)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _lib.launch(dev, what, _lib.mok_router_balance, _lib.pack_router_balance(
+        logits.data_ptr(), top_in, experts, weights, 0 if token_mask is None else token_mask.data_ptr(),
+        0 if sequence_offsets is None else sequence_offsets.data_ptr(), 0 if load is None else load.data_ptr(), losses.data_ptr(),
+        counts.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes, logits.dtype is _BF16, T, E, K, S, sigmoid))
     return losses, counts, coef
 
 
@@ -996,10 +1006,11 @@ def router_balance(logits: Tensor, top_experts: Tensor, token_mask: Tensor | Non
     [sequence_offsets[0], sequence_offsets[-1]) (int32, not decreasing; None: one sequence of all tokens).  Ids outside
     [0, E) are routes that go nowhere.  `load` (int32, the shape of counts) stands for the local counts in f: counts that
     ranks have added up.  Differentiable with respect to the logits."""
-    T, _ = _balance_logits(logits)
+    T, E = _balance_logits(logits)
     T_routes, K = _routes(top_experts)
-    _need(T_routes == T and top_experts.device == logits.device, "top_experts must have as many tokens as logits, on their device")
-    return _run_balance(logits, K, top_experts, None, None, token_mask, sequence_offsets, load, sigmoid, "router_balance")
+    if T_routes != T or top_experts.device != logits.device:
+        raise ValueError("top_experts must have as many tokens as logits, on their device")
+    return _run_balance(logits, T, E, K, top_experts.data_ptr(), 0, 0, token_mask, sequence_offsets, load, sigmoid, "router_balance")
 
 
 @_operator("mok::router_topk_balance", mutates_args=())
@@ -1009,11 +1020,14 @@ def router_topk_balance(logits: Tensor, topk: int, token_mask: Tensor | None = N
     losses, counts, coef).  With `sigmoid` the weights are the chosen experts' sigmoids over their sum.  Every token is
     routed, also those that do not count for the losses; a token without a logit above -inf gets weights of 0."""
     T, E = _balance_logits(logits)
-    _need(type(topk) is int and 0 < topk <= min(32, E), "topk must be in [1, min(32, num_experts)]")
-    experts = torch.empty(T, topk, dtype=torch.int64, device=logits.device)
-    weights = torch.empty(T, topk, dtype=torch.float32, device=logits.device)
-    return (experts, weights, *_run_balance(logits, topk, None, experts, weights, token_mask, sequence_offsets, None, sigmoid,
-                                            "router_topk_balance"))
+    if type(topk) is not int or not 0 < topk <= min(32, E):
+        raise ValueError("topk must be in [1, min(32, num_experts)]")
+    dev = logits.device
+    experts = torch.empty(T, topk, dtype=_I64, device=dev)
+    weights = torch.empty(T, topk, dtype=_F32, device=dev)
+    losses, counts, coef = _run_balance(logits, T, E, topk, 0, experts.data_ptr(), weights.data_ptr(), token_mask, sequence_offsets,
+                                        None, sigmoid, "router_topk_balance")
+    return experts, weights, losses, counts, coef
 
 
 @_operator("mok::router_balance_bwd", mutates_args=())
@@ -1024,26 +1038,34 @@ def router_balance_bwd(d_losses: Tensor, logits: Tensor, coef: Tensor, token_mas
     gradient of the router weights."""
     T, E = _balance_logits(logits)
     dev = logits.device
-    S = _sequences(T, dev, token_mask, sequence_offsets)
-    for name, t, n in (("d_losses", d_losses, 2), ("coef", coef, S * E + 2)):
-        _need(t.device == dev and tuple(t.shape) == (n,) and t.is_contiguous(), f"{name} must be contiguous [{n}] on the device of the logits")
-        _need(t.dtype == torch.float32, f"{name} must have dtype torch.float32", TypeError)
-    _need(type(sigmoid) is bool, "sigmoid must be a boolean", TypeError)
+    S = 1 if token_mask is None and sequence_offsets is None else _sequences(T, dev, token_mask, sequence_offsets)
+    for t, n in ((d_losses, 2), (coef, S * E + 2)):
+        if not (t.shape == (n,) and t.device == dev and t.is_contiguous()):
+            raise ValueError("d_losses must be contiguous [2] and coef [num_sequences * num_experts + 2], on the device of the logits")
+        if t.dtype is not _F32:
+            raise TypeError("d_losses and coef must have dtype torch.float32")
+    if type(sigmoid) is not bool:
+        raise TypeError("sigmoid must be a boolean")
+    if (top_experts is None) != (router_weights is None) or (top_experts is None) != (d_router_weights is None):
+        raise ValueError("top_experts, router_weights and d_router_weights come together or not at all")
     K = 1
-    given = [t is not None for t in (top_experts, router_weights, d_router_weights)]
-    _need(all(given) or not any(given), "top_experts, router_weights and d_router_weights come together or not at all")
-    if all(given):
+    top = w = d_w = 0
+    if top_experts is not None:
         T_routes, K = _routes(top_experts)
-        _need(T_routes == T and K <= min(32, E) and top_experts.device == dev,
-              "top_experts must be [num_tokens, topk] with topk <= min(32, num_experts), on the device of the logits")
-        for name, t in (("router_weights", router_weights), ("d_router_weights", d_router_weights)):
-            _need(t.device == dev and tuple(t.shape) == (T, K) and t.is_contiguous(), f"{name} must be contiguous and match top_experts")
-            _need(t.dtype == torch.float32, f"{name} must have dtype torch.float32", TypeError)
+        if T_routes != T or K > min(32, E) or top_experts.device != dev:
+            raise ValueError("top_experts must be [num_tokens, topk] with topk <= min(32, num_experts), on the device of the logits")
+        for t in (router_weights, d_router_weights):
+            if not (t.shape == (T, K) and t.device == dev and t.is_contiguous()):
+                raise ValueError("router_weights and d_router_weights must be contiguous and match top_experts")
+            if t.dtype is not _F32:
+                raise TypeError("router_weights and d_router_weights must have dtype torch.float32")
+        top, w, d_w = top_experts.data_ptr(), router_weights.data_ptr(), d_router_weights.data_ptr()
     d_logits = torch.empty_like(logits)
     if T > 0:
-        _lib.launch(dev, "router_balance_bwd", _lib.mok_router_balance_bwd, d_losses.data_ptr(), logits.data_ptr(),
-                    logits.dtype == torch.bfloat16, coef.data_ptr(), _vp(token_mask), _vp(sequence_offsets), _vp(top_experts),
-                    _vp(router_weights), _vp(d_router_weights), d_logits.data_ptr(), T, E, K, S, sigmoid)
+        _lib.launch(dev, "router_balance_bwd", _lib.mok_router_balance_bwd, _lib.pack_router_balance_bwd(
+            d_losses.data_ptr(), logits.data_ptr(), coef.data_ptr(), 0 if token_mask is None else token_mask.data_ptr(),
+            0 if sequence_offsets is None else sequence_offsets.data_ptr(), top, w, d_w, d_logits.data_ptr(),
+            logits.dtype is _BF16, T, E, K, S, sigmoid))
     return d_logits
 
 
@@ -1052,14 +1074,15 @@ def expert_counts(top_experts: Tensor, num_experts: int, token_mask: Tensor | No
                   sequence_offsets: Tensor | None = None) -> Tensor:
     """Routes per expert, int32 [num_sequences, num_experts], of the tokens that count (see `router_balance`).  Ids int64 or
     int32; those outside [0, num_experts) are not counted."""
-    T, K = _routes(top_experts, (torch.int64, torch.int32))
-    _need(type(num_experts) is int and 0 < num_experts <= 1024, "num_experts must be in [1, 1024]")
+    T, K = _routes(top_experts, (_I64, _I32))
+    if type(num_experts) is not int or not 0 < num_experts <= 1024:
+        raise ValueError("num_experts must be in [1, 1024]")
     dev = top_experts.device
-    S = _sequences(T, dev, token_mask, sequence_offsets)
+    S = 1 if token_mask is None and sequence_offsets is None else _sequences(T, dev, token_mask, sequence_offsets)
     if T == 0:
         return torch.zeros(S, num_experts, dtype=torch.int32, device=dev)
     counts = torch.empty(S, num_experts, dtype=torch.int32, device=dev)
-    _lib.launch(dev, "expert_counts", _lib.mok_expert_counts, top_experts.data_ptr(), top_experts.dtype == torch.int32, T, K,
+    _lib.launch(dev, "expert_counts", _lib.mok_expert_counts, top_experts.data_ptr(), top_experts.dtype is _I32, T, K,
                 num_experts, S, _vp(token_mask), _vp(sequence_offsets), counts.data_ptr())
     return counts
 
@@ -1107,18 +1130,24 @@ torch.library.register_autograd("mok::router_topk_balance", _topk_balance_backwa
 # dropout from a counter-based generator at the layer's exit (no reference op)
 # ------------------------------------------------------------------------------------------
 def _dropout_args(x: Tensor, name: str, seed: Tensor, p: float) -> None:
-    _need(x.is_cuda and x.is_contiguous(), f"{name} must be a contiguous CUDA tensor")
-    _need(x.dtype in (torch.bfloat16, torch.float32), f"{name} must have dtype torch.bfloat16 or torch.float32", TypeError)
-    _need(seed.device == x.device and tuple(seed.shape) == (1,), f"seed must have shape (1,) on the device of {name}")
-    _need(seed.dtype == torch.int64, "seed must have dtype torch.int64", TypeError)
-    _need(type(p) in (float, int) and 0 <= p <= 1, "p must be a number in [0, 1]")
+    if not (x.is_cuda and x.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous CUDA tensor")
+    if x.dtype is not _BF16 and x.dtype is not _F32:
+        raise TypeError(f"{name} must have dtype torch.bfloat16 or torch.float32")
+    if seed.dtype is not _I64:
+        raise TypeError("seed must have dtype torch.int64")
+    if seed.shape != (1,) or seed.device != x.device:
+        raise ValueError(f"seed must have shape (1,) on the device of {name}")
+    if type(p) not in (float, int) or not 0 <= p <= 1:
+        raise ValueError("p must be a number in [0, 1]")
 
 
 def _run_dropout(x: Tensor, residual: Tensor | None, seed: Tensor, p: float, what: str) -> Tensor:
     out = torch.empty_like(x)
-    if x.numel() > 0:
-        _lib.launch(x.device, what, _lib.mok_dropout_add, x.data_ptr(), _vp(residual), seed.data_ptr(), out.data_ptr(), x.numel(),
-                    x.dtype == torch.bfloat16, float(p))
+    n = x.numel()
+    if n > 0:
+        _lib.launch(x.device, what, _lib.mok_dropout_add, x.data_ptr(), None if residual is None else residual.data_ptr(),
+                    seed.data_ptr(), out.data_ptr(), n, x.dtype is _BF16, p)
     return out
 
 
@@ -1129,9 +1158,10 @@ def dropout_add(x: Tensor, residual: Tensor | None, seed: Tensor, p: float) -> T
     stored for the backward pass.  Differentiable with respect to x and residual."""
     _dropout_args(x, "x", seed, p)
     if residual is not None:
-        _need(residual.device == x.device and residual.shape == x.shape and residual.is_contiguous(),
-              "residual must be contiguous and have the shape and device of x")
-        _need(residual.dtype == x.dtype, "residual must have the dtype of x", TypeError)
+        if not (residual.shape == x.shape and residual.device == x.device and residual.is_contiguous()):
+            raise ValueError("residual must be contiguous and have the shape and device of x")
+        if residual.dtype is not x.dtype:
+            raise TypeError("residual must have the dtype of x")
     return _run_dropout(x, residual, seed, p, "dropout_add")
 
 

@@ -111,23 +111,50 @@ def test_c_entries_refuse_bad_arguments():
     from mok import _lib as L
     p = ctypes.c_void_p(4096)
     z = None
-    balance = lambda *, logits=p, T=512, E=8, K=2, S=1, top=p, out=z, w=z, off=z, n=1 << 20, scratch=p: L.mok_router_balance(  # noqa: E731
-        logits, 0, T, E, K, S, 0, top, out, w, z, off, z, p, p, p, scratch, n, z)
-    assert balance(logits=z) == balance(T=0) == balance(E=0) == balance(K=0) == balance(K=256) == balance(S=0) == -1
-    assert balance(S=2) == balance(top=z) == balance(out=p, w=p) == balance(top=z, out=p) == balance(scratch=z) == -1
-    assert balance(top=z, out=p, w=p, K=9) == balance(top=z, out=p, w=p, E=64, K=33) == -1
-    assert balance(n=64) == balance(scratch=ctypes.c_void_p(4104)) == -1
+    p = 4096
+    balance = lambda *, logits=p, T=512, E=8, K=2, S=1, top=p, out=0, w=0, off=0, n=1 << 20, scratch=p: L.mok_router_balance(  # noqa: E731
+        L.pack_router_balance(logits, top, out, w, 0, off, 0, p, p, p, scratch, n, 0, T, E, K, S, 0), None)
+    assert L.mok_router_balance(None, None) == L.mok_router_balance_bwd(None, None) == -1
+    assert balance(logits=0) == balance(T=0) == balance(E=0) == balance(K=0) == balance(K=256) == balance(S=0) == -1
+    assert balance(S=2) == balance(top=0) == balance(out=p, w=p) == balance(w=p) == balance(top=0, out=p) == balance(scratch=0) == -1
+    assert balance(top=0, out=p, w=p, K=9) == balance(top=0, out=p, w=p, E=64, K=33) == -1
+    assert balance(n=64) == balance(scratch=4104) == -1
     assert balance(E=1025) == -3 and balance(T=1 << 24, K=200) == -4
     assert L.mok_router_balance_scratch_bytes(0, 8, 1) == 0
-    bwd = lambda *, g=p, T=512, E=8, K=2, S=1, top=z, w=z, dw=z, off=z: L.mok_router_balance_bwd(                              # noqa: E731
-        g, p, 0, p, z, off, top, w, dw, p, T, E, K, S, 0, z)
-    assert bwd(g=z) == bwd(T=0) == bwd(S=3) == bwd(top=p) == bwd(top=p, w=p) == bwd(top=p, w=p, dw=p, K=33, E=64) == bwd(top=p, w=p, dw=p, K=9) == -1
+    bwd = lambda *, g=p, T=512, E=8, K=2, S=1, top=0, w=0, dw=0, off=0: L.mok_router_balance_bwd(                              # noqa: E731
+        L.pack_router_balance_bwd(g, p, p, 0, off, top, w, dw, p, 0, T, E, K, S, 0), None)
+    assert bwd(g=0) == bwd(T=0) == bwd(S=3) == bwd(top=p) == bwd(top=p, w=p) == bwd(top=p, w=p, dw=p, K=33, E=64) == -1
+    assert bwd(top=p, w=p, dw=p, K=9) == -1
     assert bwd(E=2000) == -3
+    p = ctypes.c_void_p(4096)
     counts = lambda *, ids=p, T=512, E=8, K=2, S=1, off=z: L.mok_expert_counts(ids, 0, T, K, E, S, z, off, p, z)              # noqa: E731
     assert counts(ids=z) == counts(T=-1) == counts(E=0) == counts(S=2) == -1
     assert counts(E=1025) == -3 and counts(T=1 << 30, K=4) == -4
     drop = lambda x=p, seed=p, out=p, n=8, rate=0.5: L.mok_dropout_add(x, z, seed, out, n, 1, rate, z)                         # noqa: E731
     assert drop(x=z) == drop(seed=z) == drop(out=z) == drop(n=0) == drop(n=-1) == drop(rate=1.01) == drop(rate=float("nan")) == -1
+
+
+def test_packed_arguments_have_the_layout_of_the_structs():
+    """Member by member, checked with gcc on the header: every field is set to a number of its own."""
+    import os
+    import subprocess
+    import tempfile
+    from mok import _lib as L
+    from tests.conftest import ROOT
+    text = open(os.path.join(ROOT, "include", "mok_b200.h")).read()
+    for name, pack, n in (("mok_router_balance_args", L.pack_router_balance, 18), ("mok_router_balance_bwd_args", L.pack_router_balance_bwd, 15)):
+        body = text[text.index("typedef struct " + name):]
+        body = body[body.index("{") + 1:body.index("}")]
+        fields = [w.split()[-1].strip("*") for line in body.split(";") for w in line.split(",") if w.strip()]
+        assert len(fields) == n
+        src = '#include <stdio.h>\n#include <string.h>\n#include "mok_b200.h"\nint main(){%s a; if (fread(&a, 1, sizeof a + 1, stdin) != sizeof a) return 1;' % name
+        src += "".join('printf("%%lld ", (long long)a.%s);' % f for f in fields) + "return 0;}"
+        with tempfile.TemporaryDirectory() as d:
+            c, exe = os.path.join(d, "s.c"), os.path.join(d, "s")
+            open(c, "w").write(src)
+            subprocess.check_call(["gcc", "-w", "-I", os.path.join(ROOT, "include"), c, "-o", exe])
+            out = subprocess.run([exe], input=pack(*range(1, n + 1)), capture_output=True, check=True).stdout
+        assert [int(v) for v in out.split()] == list(range(1, n + 1)), name
 
 
 # ---------------------------------------------------------------------------------------------- host side
