@@ -22,13 +22,17 @@
 namespace mok {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kRowThreads = kWarps * 32;
-// Blocks of the forward pass, all resident at once on 148 SMs: four an SM up to 256 experts, two above (their rows take twice
+constexpr int kBwdThreads = 256;
+constexpr int kSumRows = kWarps / 2;           // rows of E sums in shared memory that a block's warps share, two to a row
+// Blocks of the forward pass, all resident at once on 148 SMs: two an SM up to 256 experts, one above (their rows take twice
 // the registers).  Not read from the device: the order of the sums is the same on every GPU.
-constexpr int row_blocks_per_sm(int E) { return E <= 256 ? 4 : 2; }
-constexpr int kJoinCols = 32;
+constexpr int row_blocks_per_sm(int E) { return E <= 256 ? 2 : 1; }
+constexpr int kCluster = 8;                    // blocks of a forward pass in one launch
 constexpr unsigned kAll = 0xffffffffu;
+
+constexpr int kMinCols = 8;                    // fewest experts of a join tile
 
 struct SlotHead { float z; int rows, routes, pad; };
 
@@ -44,7 +48,7 @@ struct Scratch {
     unsigned* ticket;
     size_t bytes;
     Scratch(void* base, int slots, int E, int S) {
-        const int tiles = (E + kJoinCols - 1) / kJoinCols;
+        const int tiles = (E + kMinCols - 1) / kMinCols;
         char* at = static_cast<char*>(base);
         auto take = [&at](size_t n) { char* p = at; at += n; return p; };
         head = reinterpret_cast<SlotHead*>(take(sizeof(SlotHead) * static_cast<size_t>(slots)));
@@ -58,9 +62,21 @@ struct Scratch {
     }
 };
 
-int row_blocks(int T, int E) {
-    const int rows = kWarps * (E <= 16 ? 8 : E <= 32 ? 4 : E <= 64 ? 2 : 1);                 // that a block works on at once
-    return std::min(148 * row_blocks_per_sm(E), (T + rows - 1) / rows);
+// rows that a block works on at once
+int rows_at_once(int E) { return kWarps * (E <= 16 ? 8 : E <= 32 ? 4 : E <= 64 ? 2 : 1); }
+// One launch of one cluster, or one launch of many blocks and one that joins their slots
+bool in_one_launch(int T, int E, int S) {
+    return T <= 2 * kCluster * rows_at_once(E) && static_cast<long long>(S) * ((E + 31) / 32) <= 64;
+}
+int rows_per_block(int T, int E, int S) {
+    const int most = in_one_launch(T, E, S) ? kCluster : 148 * row_blocks_per_sm(E), at_once = rows_at_once(E);
+    const int rows = (T + most - 1) / most;
+    return (rows + at_once - 1) / at_once * at_once;
+}
+int row_blocks(int T, int E, int S) {
+    if (in_one_launch(T, E, S)) return kCluster;
+    const int rows = rows_per_block(T, E, S);
+    return (T + rows - 1) / rows;
 }
 
 // how rows of E values of `bytes` bytes at `base` can be read: chunks of eight (16 or 32 bytes), of four, or one by one
@@ -83,6 +99,7 @@ struct BalanceParams {
     float* coef;                   // [S * E] f / n_s, then 1 / S', 2 / n
     int T, E, K, S;
     int rows_per_block, blocks;
+    int one_launch;                // the blocks are one cluster and do the join themselves
     int sigmoid;
     int chunk;                     // see chunk_of
     SlotHead* head;
@@ -205,6 +222,14 @@ __device__ __forceinline__ void store_row(T* row, int e0, int E, int chunk, cons
         for (int j = 0; j < V; ++j) if (e0 + j < E) from_float(v[j], row[e0 + j]);
     }
 }
+
+// A row of values in shared memory, where every lane of a group stores and loads its own V of them four at a time: chunk-major
+// and padded by one chunk, so that neither the lanes' accesses nor those of threads that take neighbouring experts conflict.
+template <int kLanes, int V> struct SharedRow {
+    static constexpr int kFloats = V * (kLanes + 1);
+    static __device__ __forceinline__ int chunk(int lane, int j) { return ((j >> 2) * (kLanes + 1) + lane) << 2; }
+    static __device__ __forceinline__ int at(int e) { return chunk(e / V, e % V) + (e & 3); }
+};
 
 // Sequence bounds as the kernels use them: inside [0, T] whatever the caller's array holds.
 __device__ __forceinline__ int seq_bound(const int* offsets, int s, int T) {
@@ -342,9 +367,9 @@ __device__ __forceinline__ int gather_above(const float (&v)[V], float t, uint2*
     return n;
 }
 
-// One row a warp.  Let the lanes form at least K sets of `set` neighbours, and t be the least of the sets' maxima: at least K
-// values are >= t, and few more.  They are gathered, one a lane, and every lane counts those that come before its own.  Where
-// more than 32 are >= t (with K = 8 of 256 in few rows of a hundred), t is the K-th largest of the lanes' maxima instead, and
+// One row a warp.  Let the lanes form K sets of `set` neighbours, as large as they can be, and t be the least of the sets'
+// maxima: at least K values are >= t, and few more.  They are gathered, one a lane, and every lane counts those that come
+// before its own.  Where more than 32 are >= t (with K = 8 of 256 in 8 rows of 100), t is the K-th largest of the lanes' maxima instead, and
 // where that does not do either (many equal values, few above -inf, no such sets: set = 0) the row goes in rounds.
 template <int V>
 __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K, int set, uint2* gathered, float2* chosen) {
@@ -354,9 +379,8 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
     for (int j = 1; j < V; ++j) b = fmaxf(b, v[j]);
     b = b > -INFINITY ? b : -INFINITY;                             // all NaN
     float t = b;
-    if (set >= 2) t = fmaxf(t, __shfl_xor_sync(kAll, t, 1));
-    if (set >= 4) t = fmaxf(t, __shfl_xor_sync(kAll, t, 2));
-    t = warp_min(((lane | (set - 1)) + 1) * V <= E ? t : INFINITY);           // sets of lanes that are full
+    for (int off = 1; off < set; off <<= 1) t = fmaxf(t, __shfl_xor_sync(kAll, t, off));
+    t = warp_min(lane < K * set ? t : INFINITY);
     int n = 33;
     if (set > 0 && t > -INFINITY) n = gather_above(v, t, gathered);
     if (n > 32) {
@@ -391,24 +415,153 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
     __syncwarp();
 }
 
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(kAll, v); }
+
+template <int kJoinWarps> struct JoinShared {
+    float p[kJoinWarps][32], z[kJoinWarps];
+    int c[kJoinWarps][32], rows[kJoinWarps], routes[kJoinWarps];
+};
+
+// Adds the slots of a sequence for a tile of kCols experts, in an order that only depends on the sizes, and writes the tile's
+// counts, coefficients and part of the loss.  A block of kJoinWarps warps; a warp takes 32 / kCols slots at a time.
+template <int kCols, int kJoinWarps>
+__device__ __forceinline__ void join_tile(const BalanceParams& g, int index, JoinShared<kJoinWarps>& sh) {
+    constexpr int kSub = 32 / kCols;
+    const int tiles = (g.E + kCols - 1) / kCols;
+    const int s = index / tiles, tile = index - s * tiles;
+    const int begin = seq_bound(g.offsets, s, g.T), end = seq_bound(g.offsets, s + 1, g.T);
+    const int b0 = begin / g.rows_per_block, b1 = end > begin ? (end - 1) / g.rows_per_block + 1 : b0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = lane % kCols, e = tile * kCols + col;
+    float p = 0.0f, z = 0.0f;
+    int c = 0, rows = 0, routes = 0;
+#pragma unroll 4
+    for (int b = b0 + warp * kSub + lane / kCols; b < b1; b += kJoinWarps * kSub) {
+        const int4 h = __ldcg(reinterpret_cast<const int4*>(g.head + b + s));          // SlotHead
+        z += __int_as_float(h.x); rows += h.y; routes += h.z;
+        if (e < g.E) {
+            const size_t at = static_cast<size_t>(b + s) * g.E + e;
+            p += __ldcg(g.slot_p + at);
+            c += __ldcg(g.slot_routes + at);
+        }
+    }
+#pragma unroll
+    for (int off = kCols; off < 32; off <<= 1) {
+        p += __shfl_xor_sync(kAll, p, off);
+        z += __shfl_xor_sync(kAll, z, off);
+        c += __shfl_xor_sync(kAll, c, off);
+        rows += __shfl_xor_sync(kAll, rows, off);
+        routes += __shfl_xor_sync(kAll, routes, off);
+    }
+    sh.p[warp][lane] = p;
+    sh.c[warp][lane] = c;
+    if (lane == 0) { sh.z[warp] = z; sh.rows[warp] = rows; sh.routes[warp] = routes; }
+    __syncthreads();
+    if (warp == 0) {
+        const bool one = lane < kJoinWarps;
+        z = group_sum<32>(one ? sh.z[lane] : 0.0f);
+        rows = warp_sum(one ? sh.rows[lane] : 0);
+        routes = one ? sh.routes[lane] : 0;
+        if (g.load != nullptr) {
+            routes = 0;
+            for (int i = lane; i < g.E; i += 32) routes += g.load[static_cast<size_t>(s) * g.E + i];
+        }
+        routes = warp_sum(routes);
+        p = 0.0f;
+        c = 0;
+#pragma unroll
+        for (int w = lane / kCols; w < kJoinWarps; w += kSub) { p += sh.p[w][col]; c += sh.c[w][col]; }
+#pragma unroll
+        for (int off = kCols; off < 32; off <<= 1) { p += __shfl_xor_sync(kAll, p, off); c += __shfl_xor_sync(kAll, c, off); }
+        float part = 0.0f;
+        if (lane < kCols && e < g.E) {
+            const size_t at = static_cast<size_t>(s) * g.E + e;
+            g.counts[at] = c;
+            const int used = g.load != nullptr ? g.load[at] : c;
+            const float f = static_cast<float>(g.E) * static_cast<float>(used) / static_cast<float>(max(routes, 1));
+            const float a = rows > 0 ? f / static_cast<float>(rows) : 0.0f;
+            g.coef[at] = a;
+            part = a * p;
+        }
+        part = group_sum<32>(part);
+        if (lane == 0) {
+            g.part[index] = part;
+            if (tile == 0) { g.seq_z[s] = z; g.seq_rows[s] = rows; }
+        }
+    }
+}
+
+// The losses and what backward needs beside the coefficients, from the tiles' parts; one block.
+template <int kJoinWarps>
+__device__ __forceinline__ void finish(const BalanceParams& g, int parts, JoinShared<kJoinWarps>& sh) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float balance = 0.0f, z = 0.0f;
+    int live = 0, rows = 0;
+    for (int i = threadIdx.x; i < parts; i += kJoinWarps * 32) balance += __ldcg(g.part + i);
+    for (int i = threadIdx.x; i < g.S; i += kJoinWarps * 32) {
+        const int n = __ldcg(g.seq_rows + i);
+        z += __ldcg(g.seq_z + i);
+        rows += n;
+        live += n > 0;
+    }
+    balance = group_sum<32>(balance);
+    z = group_sum<32>(z);
+    rows = warp_sum(rows);
+    live = warp_sum(live);
+    __syncthreads();                           // the tile before may still be read
+    if (lane == 0) { sh.p[warp][0] = balance; sh.z[warp] = z; sh.rows[warp] = rows; sh.routes[warp] = live; }
+    __syncthreads();
+    if (warp == 0) {
+        const bool one = lane < kJoinWarps;
+        balance = group_sum<32>(one ? sh.p[lane][0] : 0.0f);
+        z = group_sum<32>(one ? sh.z[lane] : 0.0f);
+        rows = warp_sum(one ? sh.rows[lane] : 0);
+        live = warp_sum(one ? sh.routes[lane] : 0);
+        if (lane == 0) {
+            const float n = static_cast<float>(max(rows, 1)), sequences = static_cast<float>(max(live, 1));
+            g.losses[0] = balance / sequences;
+            g.losses[1] = z / n;
+            g.coef[static_cast<size_t>(g.S) * g.E] = 1.0f / sequences;
+            g.coef[static_cast<size_t>(g.S) * g.E + 1] = 2.0f / n;
+        }
+    }
+}
+
+// A block a tile; the block that finishes last does finish().  Latency-bound: a few hundred slots at most.
+template <int kCols, int kJoinWarps>
+__global__ void __launch_bounds__(kJoinWarps * 32) balance_join_kernel(const BalanceParams g) {
+    __shared__ JoinShared<kJoinWarps> sh;
+    __shared__ bool last;
+    pdl_wait();
+    join_tile<kCols>(g, blockIdx.x, sh);
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(g.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    finish(g, gridDim.x, sh);
+}
+
 // Bound by instructions.  Reads T E logits once, writes K routes a row and (p, routes) per slot.
 template <typename T, int kLanes, int V, bool kSigmoid>
 __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) balance_rows_kernel(const BalanceParams g) {
+    using Row = SharedRow<kLanes, V>;
     constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // chosen experts a lane, at most (K <= 32 and <= E)
-    extern __shared__ float smem[];                            // p [kWarps][E], routes [E], then the chosen (value, expert) [kGroups][K]
+    extern __shared__ __align__(16) float smem[];               // sums of p [kSumRows], routes [E], then the chosen (value, expert) [kGroups][K]
     __shared__ alignas(16) uint2 s_gathered[kLanes == 32 ? kWarps : 1][32];
     __shared__ float s_z[kWarps];
     __shared__ int s_rows[kWarps], s_routes;
-    int* const hist = reinterpret_cast<int*>(smem + static_cast<size_t>(kWarps) * g.E);
+    int* const hist = reinterpret_cast<int*>(smem + kSumRows * Row::kFloats);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes;
     float2* const chosen = reinterpret_cast<float2*>(hist + ((g.E + 1) & ~1)) + static_cast<size_t>(group) * g.K;
     const int e0 = l * V;
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
     const bool select = g.top_in == nullptr;
-    const int full = g.E / V;                                  // lanes that hold V values (select_by_rank: sets of 4, 2 or 1 of them)
-    const int set = full / 4 >= g.K ? 4 : full / 2 >= g.K ? 2 : full >= g.K ? 1 : 0;
+    int set = 32;                                              // select_by_rank: the largest sets of lanes of which there are K
+    while (set > 0 && (g.E + set * V / 2) / (set * V) < g.K) set >>= 1;         // (one that is half full counts)
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
@@ -482,12 +635,23 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
             }
         }
         if (counted) {
-            float* const mine = smem + static_cast<size_t>(warp) * g.E;
+            float* const mine = smem + (warp % kSumRows) * Row::kFloats;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
+            for (int j = 0; j < V; j += 4) {
 #pragma unroll
-                for (int off = kLanes; off < 32; off <<= 1) acc[j] += __shfl_xor_sync(kAll, acc[j], off);
-                if (lane < kLanes && e0 + j < g.E) mine[e0 + j] = acc[j];
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int off = kLanes; off < 32; off <<= 1) acc[j + i] += __shfl_xor_sync(kAll, acc[j + i], off);
+                if (warp >= kSumRows && lane < kLanes)
+                    *reinterpret_cast<float4*>(mine + Row::chunk(l, j)) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < V; j += 4) {
+                if (warp < kSumRows && lane < kLanes) {
+                    float4& x = *reinterpret_cast<float4*>(mine + Row::chunk(l, j));
+                    x = make_float4(x.x + acc[j], x.y + acc[j + 1], x.z + acc[j + 2], x.w + acc[j + 3]);
+                }
             }
 #pragma unroll
             for (int off = kLanes; off < 32; off <<= 1) { z += __shfl_xor_sync(kAll, z, off); rows += __shfl_xor_sync(kAll, rows, off); }
@@ -495,12 +659,22 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
             if (lane == 0) { s_z[warp] = z; s_rows[warp] = rows; }
             __syncthreads();
             const size_t slot = static_cast<size_t>(blockIdx.x) + s;
-            for (int e = threadIdx.x; e < g.E; e += kRowThreads) {
-                float sum = 0.0f;
+            for (int e = threadIdx.x * 4; e < g.E; e += kRowThreads * 4) {
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) sum += smem[static_cast<size_t>(w) * g.E + e];
-                g.slot_p[slot * g.E + e] = sum;
-                g.slot_routes[slot * g.E + e] = hist[e];
+                for (int w = 0; w < kSumRows; ++w) {
+                    const float4 x = *reinterpret_cast<const float4*>(smem + w * Row::kFloats + Row::at(e));
+                    sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
+                }
+                float* const to_p = g.slot_p + slot * g.E + e;
+                int* const to_routes = g.slot_routes + slot * g.E + e;
+                if (g.E % 4 == 0) {
+                    *reinterpret_cast<float4*>(to_p) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                    *reinterpret_cast<int4*>(to_routes) = make_int4(hist[e], hist[e + 1], hist[e + 2], hist[e + 3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (e + i < g.E) { to_p[i] = sum[i]; to_routes[i] = hist[e + i]; }
+                }
             }
             if (threadIdx.x == 0) {
                 SlotHead h{0.0f, 0, s_routes, 0};
@@ -512,91 +686,15 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
         }
         pos = end;
     }
-}
-
-__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(kAll, v); }
-
-// One block per 32 experts of a sequence, one lane per expert; its warps take the sequence's slots in turn, and their sums
-// are added in warp order.  The block that finishes last adds up the losses.  Latency-bound: a few hundred slots at most.
-template <int kJoinWarps>
-__global__ void __launch_bounds__(kJoinWarps * 32) balance_join_kernel(const BalanceParams g) {
-    __shared__ float s_p[kJoinWarps][kJoinCols], s_z[kJoinWarps], s_balance[kJoinWarps];
-    __shared__ int s_c[kJoinWarps][kJoinCols], s_rows[kJoinWarps], s_routes[kJoinWarps];
-    __shared__ bool last;
-    pdl_wait();
-    const int tiles = (g.E + kJoinCols - 1) / kJoinCols;
-    const int s = blockIdx.x / tiles, tile = blockIdx.x - s * tiles;
-    const int begin = seq_bound(g.offsets, s, g.T), end = seq_bound(g.offsets, s + 1, g.T);
-    const int b0 = begin / g.rows_per_block, b1 = end > begin ? (end - 1) / g.rows_per_block + 1 : b0;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = tile * kJoinCols + lane;
-    float p = 0.0f, z = 0.0f;
-    int c = 0, rows = 0, routes = 0;
-#pragma unroll 4
-    for (int b = b0 + warp; b < b1; b += kJoinWarps) {
-        const SlotHead h = g.head[b + s];
-        z += h.z; rows += h.rows; routes += h.routes;
-        if (e < g.E) {
-            const size_t at = static_cast<size_t>(b + s) * g.E + e;
-            p += g.slot_p[at];
-            c += g.slot_routes[at];
-        }
-    }
-    s_p[warp][lane] = p;
-    s_c[warp][lane] = c;
-    if (lane == 0) { s_z[warp] = z; s_rows[warp] = rows; s_routes[warp] = routes; }
+    if (!g.one_launch) return;
+    JoinShared<kWarps>& sh = *reinterpret_cast<JoinShared<kWarps>*>(smem);
+    const int parts = g.S * ((g.E + 31) / 32);
     __syncthreads();
-    if (warp == 0) {
-        if (lane < kJoinWarps) { z = s_z[lane]; rows = s_rows[lane]; routes = s_routes[lane]; } else { z = 0.0f; rows = 0; routes = 0; }
-        z = group_sum<32>(z);
-        rows = warp_sum(rows);
-        if (g.load != nullptr) {
-            routes = 0;
-            for (int i = lane; i < g.E; i += 32) routes += g.load[static_cast<size_t>(s) * g.E + i];
-        }
-        routes = warp_sum(routes);
-#pragma unroll
-        for (int w = 1; w < kJoinWarps; ++w) { p += s_p[w][lane]; c += s_c[w][lane]; }
-        float part = 0.0f;
-        if (e < g.E) {
-            const size_t at = static_cast<size_t>(s) * g.E + e;
-            g.counts[at] = c;
-            const int used = g.load != nullptr ? g.load[at] : c;
-            const float f = static_cast<float>(g.E) * static_cast<float>(used) / static_cast<float>(max(routes, 1));
-            const float a = rows > 0 ? f / static_cast<float>(rows) : 0.0f;
-            g.coef[at] = a;
-            part = a * p;
-        }
-        part = group_sum<32>(part);
-        if (lane == 0) {
-            g.part[blockIdx.x] = part;
-            if (tile == 0) { g.seq_z[s] = z; g.seq_rows[s] = rows; }
-            __threadfence();
-            last = atomicAdd(g.ticket, 1u) == gridDim.x - 1;
-        }
-    }
+    cluster_sync_all();                        // every slot is written
+    for (int i = blockIdx.x; i < parts; i += gridDim.x) { __syncthreads(); join_tile<32>(g, i, sh); }
     __syncthreads();
-    if (!last) return;
-    __threadfence();
-    float balance = 0.0f;
-    z = 0.0f;
-    int live = 0;
-    rows = 0;
-    for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kJoinWarps * 32) balance += __ldcg(&g.part[i]);
-    for (int i = threadIdx.x; i < g.S; i += kJoinWarps * 32) { const int n = __ldcg(&g.seq_rows[i]); z += __ldcg(&g.seq_z[i]); rows += n; live += n > 0; }
-    balance = group_sum<32>(balance);
-    z = group_sum<32>(z);
-    rows = warp_sum(rows);
-    live = warp_sum(live);
-    if (lane == 0) { s_balance[warp] = balance; s_z[warp] = z; s_rows[warp] = rows; s_routes[warp] = live; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kJoinWarps; ++w) { balance += s_balance[w]; z += s_z[w]; rows += s_rows[w]; live += s_routes[w]; }
-        const float n = static_cast<float>(max(rows, 1)), sequences = static_cast<float>(max(live, 1));
-        g.losses[0] = balance / sequences;
-        g.losses[1] = z / n;
-        g.coef[static_cast<size_t>(g.S) * g.E] = 1.0f / sequences;
-        g.coef[static_cast<size_t>(g.S) * g.E + 1] = 2.0f / n;
-    }
+    cluster_sync_all();
+    if (blockIdx.x == 0) finish(g, parts, sh);
 }
 
 struct BalanceBwdParams {
@@ -617,14 +715,15 @@ struct BalanceBwdParams {
 // gradient is p c: two operations a value once the sums are there.  The gradient of the chosen weights is scattered into a row
 // of shared memory, K values, and picked up by the lanes that hold their experts.
 template <typename T, int kLanes, int V, bool kSigmoid>
-__global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceBwdParams g) {
-    constexpr int kGroups = kRowThreads / kLanes;
+__global__ void __launch_bounds__(kBwdThreads) balance_bwd_kernel(const BalanceBwdParams g) {
+    constexpr int kGroups = kBwdThreads / kLanes;
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // routes a lane, at most (topk <= 32 and <= E)
-    __shared__ alignas(16) float s_add[kGroups][kLanes * V];
+    using Row = SharedRow<kLanes, V>;
+    __shared__ alignas(16) float s_add[kGroups][Row::kFloats];
     const int lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes, e0 = l * V;
     float* const add = s_add[group];
 #pragma unroll
-    for (int j = 0; j < V; ++j) add[e0 + j] = 0.0f;
+    for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(add + Row::chunk(l, j)) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     pdl_wait();
     const size_t scalars = static_cast<size_t>(g.S) * g.E;
     const float gb = g.d_losses[0] * g.coef[scalars], gz = g.d_losses[1] * g.coef[scalars + 1];
@@ -701,7 +800,10 @@ __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceB
             for (int i = 0; i < kPer; ++i) {
                 dw[i] = w[i] == 0.0f ? 0.0f : w[i] * (dw[i] - dot);
                 if (kSigmoid && expert[i] >= 0) dw[i] *= sigmoid_rest(to_float(row[expert[i]]));
-                if (expert[i] >= 0) add[expert[i]] = __int_as_float(l + i * kLanes);
+                if (expert[i] >= 0) {
+                    expert[i] = Row::at(expert[i]);                // from here on its place in the shared row
+                    add[expert[i]] = __int_as_float(l + i * kLanes);
+                }
             }
             // an expert that a row names twice (finished routes may) shows in the tag that was overwritten
             bool twice = false;
@@ -725,7 +827,7 @@ __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceB
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < V; j += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(add + e0 + j);
+                const float4 x = *reinterpret_cast<const float4*>(add + Row::chunk(l, j));
                 d[j] += x.x; d[j + 1] += x.y; d[j + 2] += x.z; d[j + 3] += x.w;
             }
             __syncwarp();
@@ -737,56 +839,81 @@ __global__ void __launch_bounds__(kRowThreads) balance_bwd_kernel(const BalanceB
     }
 }
 
+constexpr int kCountThreads = 512;
 struct CountParams {
     const void* top;
     int ids_i32;
     const uint8_t* mask;
     const int* offsets;
-    int* counts;                   // [S, E], zeroed
+    int* counts;                   // [S, E], zeroed before a launch of several blocks
     int T, E, K, S, rows_per_block;
 };
 
 // Each block counts a run of rows in shared memory, sequence by sequence, and adds what it found: integer sums do not
-// depend on their order.  Reads T K ids.
-__global__ void __launch_bounds__(kRowThreads) expert_counts_kernel(const CountParams g) {
+// depend on their order.  One block alone stores instead, and clears the counts of sequences without rows itself.  Reads T K
+// ids.
+__global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const CountParams g) {
     extern __shared__ int bins[];
     pdl_wait();
+    const bool alone = gridDim.x == 1;
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
-    for (int s = first_sequence(g.offsets, g.S, pos, g.T); s < g.S && pos < hi; ++s) {
+    const unsigned topk = g.K;
+    for (int s = alone ? 0 : first_sequence(g.offsets, g.S, pos, g.T); s < g.S && (alone || pos < hi); ++s) {
         const int begin = max(seq_bound(g.offsets, s, g.T), pos), end = min(seq_bound(g.offsets, s + 1, g.T), hi);
-        if (begin >= hi) break;
-        if (end <= begin) continue;
-        for (int e = threadIdx.x; e < g.E; e += kRowThreads) bins[e] = 0;
+        if (!alone && begin >= hi) break;
+        if (!alone && end <= begin) continue;
+        for (int e = threadIdx.x; e < g.E; e += kCountThreads) bins[e] = 0;
         __syncthreads();
-        const long long stop = static_cast<long long>(end) * g.K;
-        for (long long i = static_cast<long long>(begin) * g.K + threadIdx.x; i < stop; i += kRowThreads) {
-            if (g.mask != nullptr && !g.mask[i / g.K]) continue;
-            const long long e = g.ids_i32 ? static_cast<const int*>(g.top)[i] : static_cast<const long long*>(g.top)[i];
-            if (e >= 0 && e < g.E) atomicAdd(&bins[e], 1);
+        if (end > begin) {
+            const size_t at = static_cast<size_t>(begin) * topk;
+            const unsigned n = static_cast<unsigned>(end - begin) * topk;          // a call has fewer than 2^31 routes
+#pragma unroll 4
+            for (unsigned i = threadIdx.x; i < n; i += kCountThreads) {
+                const long long e = g.ids_i32 ? static_cast<const int*>(g.top)[at + i] : static_cast<const long long*>(g.top)[at + i];
+                if (e >= 0 && e < g.E && (g.mask == nullptr || g.mask[begin + i / topk])) atomicAdd(&bins[e], 1);
+            }
+            pos = end;
         }
         __syncthreads();
-        for (int e = threadIdx.x; e < g.E; e += kRowThreads)
-            if (bins[e]) atomicAdd(&g.counts[static_cast<size_t>(s) * g.E + e], bins[e]);
+        int* const out = g.counts + static_cast<size_t>(s) * g.E;
+        for (int e = threadIdx.x; e < g.E; e += kCountThreads) {
+            if (alone) out[e] = bins[e];
+            else if (bins[e]) atomicAdd(out + e, bins[e]);
+        }
         __syncthreads();
-        pos = end;
     }
 }
 
 template <typename T, int kLanes, int V, bool kSigmoid>
 int launch_rows(const BalanceParams& p, cudaStream_t s) {
     const size_t chosen = p.top_in == nullptr ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
-    const size_t smem = (static_cast<size_t>(kWarps) * p.E + ((p.E + 1) & ~1) + chosen) * 4;
-    return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid>, p.blocks, kRowThreads, smem, s, false, true, p);
+    const size_t smem = std::max((static_cast<size_t>(kSumRows) * SharedRow<kLanes, V>::kFloats + ((p.E + 1) & ~1) + chosen) * 4, sizeof(JoinShared<kWarps>));
+    if (!p.one_launch) return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid>, p.blocks, kRowThreads, smem, s, false, true, p);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kCluster);
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    auto* kern = balance_rows_kernel<T, kLanes, V, kSigmoid>;
+    MOK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+    return MOK_OK;
 }
 
 template <typename T, int kLanes, int V, bool kSigmoid>
 int launch_bwd(BalanceBwdParams p, cudaStream_t s) {
-    constexpr int kGroups = kRowThreads / kLanes;
+    constexpr int kGroups = kBwdThreads / kLanes;
     const int blocks = std::min((p.T + kGroups - 1) / kGroups, device_sm_count() * 8);
     p.rows_per_block = (p.T + blocks - 1) / blocks;
-    return launch_kernel(balance_bwd_kernel<T, kLanes, V, kSigmoid>, blocks, kRowThreads, 0, s, false, true, p);
+    return launch_kernel(balance_bwd_kernel<T, kLanes, V, kSigmoid>, blocks, kBwdThreads, 0, s, false, true, p);
 }
 
 // lanes a row and values a lane: four values where a row fits, so that 32 lanes hold several short rows
@@ -811,7 +938,7 @@ using namespace mok;
 
 extern "C" size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences) {
     if (bad_sizes(num_tokens, num_experts, 1, num_sequences)) return 0;
-    return Scratch(nullptr, row_blocks(num_tokens, num_experts) + num_sequences, num_experts, num_sequences).bytes;
+    return Scratch(nullptr, row_blocks(num_tokens, num_experts, num_sequences) + num_sequences, num_experts, num_sequences).bytes;
 }
 
 extern "C" int mok_router_balance(const mok_router_balance_args* args, void* stream) {
@@ -823,10 +950,10 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
     if (!a.top_experts_in && (K > 32 || K > E)) return MOK_ERR_INVALID;
     if (!a.sequence_offsets && S != 1) return MOK_ERR_INVALID;
     if (E > 1024) return MOK_ERR_UNSUPPORTED;
-    const int tiles = (E + kJoinCols - 1) / kJoinCols;
-    if (too_many_routes(T, K) || static_cast<long long>(S) * tiles > 0x3fffffff) return MOK_ERR_TOO_LARGE;
+    if (too_many_routes(T, K) || static_cast<long long>(S) * E > 0x7fffffff) return MOK_ERR_TOO_LARGE;
     BalanceParams p{};
-    p.blocks = row_blocks(T, E);
+    p.blocks = row_blocks(T, E, S);
+    p.one_launch = in_one_launch(T, E, S);
     const Scratch at(a.scratch, p.blocks + S, E, S);
     if (a.scratch_bytes < at.bytes || reinterpret_cast<uintptr_t>(a.scratch) % 16) return MOK_ERR_INVALID;
     p.logits = a.logits;
@@ -840,13 +967,13 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
     p.counts = a.counts;
     p.coef = a.coef;
     p.T = T; p.E = E; p.K = K; p.S = S;
-    p.rows_per_block = (T + p.blocks - 1) / p.blocks;
+    p.rows_per_block = rows_per_block(T, E, S);
     p.sigmoid = a.sigmoid;
     p.chunk = chunk_of(a.logits, E, a.logits_bf16 ? 2 : 4);
     p.head = at.head; p.slot_p = at.p; p.slot_routes = at.routes; p.part = at.part; p.seq_z = at.seq_z; p.seq_rows = at.seq_rows;
     p.ticket = at.ticket;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    ProfScope prof(kSlotOther, s, 2);
+    ProfScope prof(kSlotOther, s, p.one_launch ? 1 : 2);
     int rc;
     if (a.logits_bf16) {
 #define MOK_CALL(lanes, v) (p.sigmoid ? launch_rows<__nv_bfloat16, lanes, v, true>(p, s) : launch_rows<__nv_bfloat16, lanes, v, false>(p, s))
@@ -857,10 +984,10 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
         rc = MOK_ROW_SHAPE(E, MOK_CALL);
 #undef MOK_CALL
     }
-    if (rc != MOK_OK) return rc;
-    // warps for the slots of a sequence, on average
-    if (p.blocks / S >= 64) return launch_kernel(balance_join_kernel<32>, S * tiles, 1024, 0, s, false, true, p);
-    return launch_kernel(balance_join_kernel<8>, S * tiles, 256, 0, s, false, true, p);
+    if (rc != MOK_OK || p.one_launch) return rc;
+    // few sequences: narrow tiles and many warps, each sequence has many slots; many: wide tiles, few slots each
+    if (S <= 4) return launch_kernel(balance_join_kernel<8, 32>, S * ((E + 7) / 8), 1024, 0, s, false, true, p);
+    return launch_kernel(balance_join_kernel<32, 8>, S * ((E + 31) / 32), 256, 0, s, false, true, p);
 }
 
 extern "C" int mok_router_balance_bwd(const mok_router_balance_bwd_args* args, void* stream) {
@@ -894,11 +1021,13 @@ extern "C" int mok_expert_counts(const void* top_experts, int ids_i32, int num_t
     if (!sequence_offsets && num_sequences != 1) return MOK_ERR_INVALID;
     if (num_experts > 1024) return MOK_ERR_UNSUPPORTED;
     if (too_many_routes(num_tokens, topk)) return MOK_ERR_TOO_LARGE;
-    const int blocks = std::min((num_tokens + 63) / 64, device_sm_count() * 4);
+    const long long routes = static_cast<long long>(num_tokens) * topk;
+    const bool alone = routes <= 8192 && num_sequences <= 8;
+    const int blocks = alone ? 1 : static_cast<int>(std::min<long long>((routes + 4095) / 4096, device_sm_count() * 4));
     CountParams p{top_experts, ids_i32, token_mask, sequence_offsets, counts, num_tokens, num_experts, topk, num_sequences,
                   (num_tokens + blocks - 1) / blocks};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(kSlotOther, s);
-    MOK_CUDA_CHECK(cudaMemsetAsync(counts, 0, static_cast<size_t>(num_sequences) * num_experts * 4, s));
-    return launch_kernel(expert_counts_kernel, blocks, kRowThreads, static_cast<size_t>(num_experts) * 4, s, false, false, p);
+    if (!alone) MOK_CUDA_CHECK(cudaMemsetAsync(counts, 0, static_cast<size_t>(num_sequences) * num_experts * 4, s));
+    return launch_kernel(expert_counts_kernel, blocks, kCountThreads, static_cast<size_t>(num_experts) * 4, s, false, alone, p);
 }
