@@ -171,7 +171,7 @@ int mok_router_topk_bwd(const int32_t* top_experts_i32, const float* router_weig
  * first among equals) into top_experts_out int64 and router_weights f32 [T, K] (softmax, or sigmas over their sum, of those K).
  * load: int32 [num_sequences, E] that stands for the counts in f (NULL: the counts).  Outputs: losses f32 [2], counts int32
  * [num_sequences, E], coef f32 [num_sequences * E + 2] for mok_router_balance_bwd.  scratch: 16-byte aligned,
- * mok_router_balance_scratch_bytes bytes, of this call alone until it has run.
+ * mok_router_balance_scratch_bytes bytes (0: none is needed, NULL will do), of this call alone until it has run.
  * mok_router_balance_bwd writes all of d_logits (type of logits) from d_losses f32 [2] and, where the three are not NULL,
  * from the gradient of the router weights (topk <= 32 and <= num_experts).
  * No reference counterpart (the reference takes finished routes and returns no losses). */

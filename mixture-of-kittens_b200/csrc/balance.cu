@@ -25,10 +25,16 @@ namespace {
 constexpr int kWarps = 16;
 constexpr int kRowThreads = kWarps * 32;
 constexpr int kBwdThreads = 256;
+// Blocks of the backward pass that an SM has to be able to hold, which bounds their registers; the grid is twice as many.
+// One B200, us: 131072 x 256 f32 with five 53, four 58, six 55; 65536 x 500 bf16 with four 56, two 70, sigmoid scores 30000 x 500
+// with three 36, four (spills) 44; 30000 x 1024 f32 with two 63, three (spills) 88 to 92.
+constexpr int bwd_blocks_per_sm(int V, bool sigmoid) { return V <= 8 ? 5 : V == 16 ? 4 - sigmoid : 2; }
 constexpr int kSumRows = kWarps / 2;           // rows of E sums in shared memory that a block's warps share, two to a row
-// Blocks of the forward pass, all resident at once on 148 SMs: two an SM up to 256 experts, one above (their rows take twice
+// Blocks of the forward pass, all resident at once on 148 SMs: two an SM up to 512 experts, one above (their rows take twice
 // the registers).  Not read from the device: the order of the sums is the same on every GPU.
-constexpr int row_blocks_per_sm(int E) { return E <= 256 ? 2 : 1; }
+constexpr int row_blocks_per_sm(int E) { return E <= 512 ? 2 : 1; }
+
+
 constexpr int kCluster = 8;                    // blocks of a forward pass in one launch
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -64,10 +70,10 @@ struct Scratch {
 
 // rows that a block works on at once
 int rows_at_once(int E) { return kWarps * (E <= 16 ? 8 : E <= 32 ? 4 : E <= 64 ? 2 : 1); }
-// One launch of one cluster, or one launch of many blocks and one that joins their slots
-bool in_one_launch(int T, int E, int S) {
-    return T <= 2 * kCluster * rows_at_once(E) && static_cast<long long>(S) * ((E + 31) / 32) <= 64;
-}
+// One launch of one cluster that joins its blocks' sums through shared memory and needs no scratch, or one launch of many
+// blocks and one that joins their slots.  Up to two rows a group of lanes the cluster saves the caller a launch and an
+// allocation, 4 us of its time; the device takes 6.5 us for one row a group and 7.1 to 9.8 for two, against 7 to 9.5 with two launches.
+bool in_one_launch(int T, int E, int S) { return S == 1 && T <= 2 * kCluster * rows_at_once(E); }
 int rows_per_block(int T, int E, int S) {
     const int most = in_one_launch(T, E, S) ? kCluster : 148 * row_blocks_per_sm(E), at_once = rows_at_once(E);
     const int rows = (T + most - 1) / most;
@@ -223,6 +229,26 @@ __device__ __forceinline__ void store_row(T* row, int e0, int E, int chunk, cons
     }
 }
 
+// another block's copy of a shared-memory object of this cluster
+__device__ __forceinline__ uint32_t remote_shared(const void* p, int block) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(block));
+    return at;
+}
+__device__ __forceinline__ float remote_load(const float* p, int block) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote_shared(p, block)) : "memory");
+    return v;
+}
+__device__ __forceinline__ int remote_load(const int* p, int block) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote_shared(p, block)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void remote_store(float* p, int block, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote_shared(p, block)), "f"(v) : "memory");
+}
+
 // A row of values in shared memory, where every lane of a group stores and loads its own V of them four at a time: chunk-major
 // and padded by one chunk, so that neither the lanes' accesses nor those of threads that take neighbouring experts conflict.
 template <int kLanes, int V> struct SharedRow {
@@ -236,10 +262,19 @@ __device__ __forceinline__ int seq_bound(const int* offsets, int s, int T) {
     if (offsets == nullptr) return s ? T : 0;
     return min(max(offsets[s], 0), T);
 }
-// first sequence that ends behind row `row` (S if none)
+// First sequence that ends behind row `row` (S if none); a whole warp searches, 32 sequences at a time.
 __device__ __forceinline__ int first_sequence(const int* offsets, int S, int row, int T) {
-    int lo = 0, hi = S;
-    while (lo < hi) { const int mid = (lo + hi) >> 1; if (seq_bound(offsets, mid + 1, T) > row) hi = mid; else lo = mid + 1; }
+    if (offsets == nullptr) return 0;
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = S;
+    while (n > 0) {
+        const int step = (n + 31) / 32, probe = lo + lane * step;
+        const bool before = probe < lo + n && seq_bound(offsets, probe + 1, T) <= row;
+        const int passed = __popc(__ballot_sync(kAll, before));
+        const int hi = min(lo + passed * step, lo + n);            // ends behind the row, or the end of the range
+        if (passed > 0) lo += (passed - 1) * step + 1;
+        n = passed > 0 ? hi - lo : 0;
+    }
     return lo;
 }
 
@@ -417,6 +452,17 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
 
 __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(kAll, v); }
 
+__device__ __forceinline__ float expert_share(int E, int routes, int of) {
+    return static_cast<float>(E) * static_cast<float>(routes) / static_cast<float>(max(of, 1));
+}
+__device__ __forceinline__ void write_losses(const BalanceParams& g, float balance, float z, int rows, int live) {
+    const float n = static_cast<float>(max(rows, 1)), sequences = static_cast<float>(max(live, 1));
+    g.losses[0] = balance / sequences;
+    g.losses[1] = z / n;
+    g.coef[static_cast<size_t>(g.S) * g.E] = 1.0f / sequences;
+    g.coef[static_cast<size_t>(g.S) * g.E + 1] = 2.0f / n;
+}
+
 template <int kJoinWarps> struct JoinShared {
     float p[kJoinWarps][32], z[kJoinWarps];
     int c[kJoinWarps][32], rows[kJoinWarps], routes[kJoinWarps];
@@ -477,8 +523,7 @@ __device__ __forceinline__ void join_tile(const BalanceParams& g, int index, Joi
             const size_t at = static_cast<size_t>(s) * g.E + e;
             g.counts[at] = c;
             const int used = g.load != nullptr ? g.load[at] : c;
-            const float f = static_cast<float>(g.E) * static_cast<float>(used) / static_cast<float>(max(routes, 1));
-            const float a = rows > 0 ? f / static_cast<float>(rows) : 0.0f;
+            const float a = rows > 0 ? expert_share(g.E, used, routes) / static_cast<float>(rows) : 0.0f;
             g.coef[at] = a;
             part = a * p;
         }
@@ -517,11 +562,7 @@ __device__ __forceinline__ void finish(const BalanceParams& g, int parts, JoinSh
         rows = warp_sum(one ? sh.rows[lane] : 0);
         live = warp_sum(one ? sh.routes[lane] : 0);
         if (lane == 0) {
-            const float n = static_cast<float>(max(rows, 1)), sequences = static_cast<float>(max(live, 1));
-            g.losses[0] = balance / sequences;
-            g.losses[1] = z / n;
-            g.coef[static_cast<size_t>(g.S) * g.E] = 1.0f / sequences;
-            g.coef[static_cast<size_t>(g.S) * g.E + 1] = 2.0f / n;
+            write_losses(g, balance, z, rows, live);
         }
     }
 }
@@ -543,29 +584,35 @@ __global__ void __launch_bounds__(kJoinWarps * 32) balance_join_kernel(const Bal
     finish(g, gridDim.x, sh);
 }
 
-// Bound by instructions.  Reads T E logits once, writes K routes a row and (p, routes) per slot.
+// Bound by instructions and, without the choice, by the latency of its loads.  Reads T E logits once, writes K routes a row and (p,
+// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 79 (21), finished routes
+// 44; 65536 x 500 bf16, K = 6, 61 sequences: 70 (10) and 43; 16384 x 128: 16 (1.3) and 11.  A row of 256 takes 500 instructions
+// with the choice, 180 without; in rounds of one maximum each the choice alone took 540.  Loading the next row ahead: 53 -> 44
+// without the choice at 256 experts; above, the registers it takes cost a block an SM (44 -> 59 at 500).
 template <typename T, int kLanes, int V, bool kSigmoid>
 __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) balance_rows_kernel(const BalanceParams g) {
     using Row = SharedRow<kLanes, V>;
+    constexpr bool kAhead = V <= 8;            // the next row is loaded while this one is worked on
     constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // chosen experts a lane, at most (K <= 32 and <= E)
     extern __shared__ __align__(16) float smem[];               // sums of p [kSumRows], routes [E], then the chosen (value, expert) [kGroups][K]
     __shared__ alignas(16) uint2 s_gathered[kLanes == 32 ? kWarps : 1][32];
-    __shared__ float s_z[kWarps];
+    __shared__ float s_z[kWarps], s_part[kWarps], s_parts[kCluster];
     __shared__ int s_rows[kWarps], s_routes;
     int* const hist = reinterpret_cast<int*>(smem + kSumRows * Row::kFloats);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes;
     float2* const chosen = reinterpret_cast<float2*>(hist + ((g.E + 1) & ~1)) + static_cast<size_t>(group) * g.K;
     const int e0 = l * V;
     pdl_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *g.ticket = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && !g.one_launch) *g.ticket = 0;
     const bool select = g.top_in == nullptr;
     int set = 32;                                              // select_by_rank: the largest sets of lanes of which there are K
     while (set > 0 && (g.E + set * V / 2) / (set * V) < g.K) set >>= 1;         // (one that is half full counts)
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
-    int s = g.offsets == nullptr ? 0 : first_sequence(g.offsets, g.S, pos, g.T);
+    int s = first_sequence(g.offsets, g.S, pos, g.T);
+    bool summed = false;
     while (pos < hi) {
         // the next run of rows: a sequence's, or rows between and behind the sequences
         const int begin = s < g.S ? max(seq_bound(g.offsets, s, g.T), pos) : hi;
@@ -582,23 +629,25 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] = 0.0f;
         // all lanes of a warp stay in step; groups past the run work on nothing
-        for (int t0 = pos + warp * (32 / kLanes); t0 < end && (counted || select); t0 += kGroups) {
+        auto load = [&](int t0, float (&v)[V]) {
+            load_row<V>(static_cast<const T*>(g.logits) + static_cast<size_t>(min(t0 + lane / kLanes, end - 1)) * g.E, e0, g.E, g.chunk, -INFINITY, v);
+        };
+        float next[V];
+        const int t_first = pos + warp * (32 / kLanes);
+        if (kAhead && t_first < end && (counted || select)) load(t_first, next);
+        for (int t0 = t_first; t0 < end && (counted || select); t0 += kGroups) {
             const int t = t0 + lane / kLanes;
             const bool there = t < end;
             float v[V];
-            load_row<V>(static_cast<const T*>(g.logits) + static_cast<size_t>(there ? t : t0) * g.E, e0, g.E, g.chunk, -INFINITY, v);
+            if constexpr (kAhead) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = next[j];
+                if (t0 + kGroups < end) load(t0 + kGroups, next);
+            } else {
+                load(t0, v);
+            }
             const bool live = there && counted && (g.mask == nullptr || g.mask[t]);
             const size_t o = static_cast<size_t>(t) * g.K;
-            if (counted) {
-                float ex[V], sg[V];
-                const RowStats r = row_stats<kLanes, V, kSigmoid>(v, ex, sg);
-                if (live) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) acc[j] = kSigmoid ? fmaf(sg[j], r.inv_sg, acc[j]) : fmaf(ex[j], r.inv, acc[j]);
-                    z = fmaf(r.lse, r.lse, z);
-                    ++rows;
-                }
-            }
             if (select) {
                 if constexpr (kLanes == 32) select_by_rank<V>(v, g.E, g.K, set, s_gathered[warp], chosen);
                 else select_in_rounds<kLanes, V>(v, g.E, g.K, chosen);
@@ -633,6 +682,16 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
                     if (e >= 0 && e < g.E) { atomicAdd(&hist[e], 1); ++routes; }
                 }
             }
+            if (counted) {
+                float ex[V], sg[V];
+                const RowStats r = row_stats<kLanes, V, kSigmoid>(v, ex, sg);
+                if (live) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[j] = kSigmoid ? fmaf(sg[j], r.inv_sg, acc[j]) : fmaf(ex[j], r.inv, acc[j]);
+                    z = fmaf(r.lse, r.lse, z);
+                    ++rows;
+                }
+            }
         }
         if (counted) {
             float* const mine = smem + (warp % kSumRows) * Row::kFloats;
@@ -659,12 +718,16 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
             if (lane == 0) { s_z[warp] = z; s_rows[warp] = rows; }
             __syncthreads();
             const size_t slot = static_cast<size_t>(blockIdx.x) + s;
-            for (int e = threadIdx.x * 4; e < g.E; e += kRowThreads * 4) {
+            for (int e = threadIdx.x * 4; e < g.E; e += kRowThreads * 4) {     // (once: a block has at least 256 threads)
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int w = 0; w < kSumRows; ++w) {
                     const float4 x = *reinterpret_cast<const float4*>(smem + w * Row::kFloats + Row::at(e));
                     sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
+                }
+                if (g.one_launch) {                                // stays here: only this thread reads these places of the rows
+                    *reinterpret_cast<float4*>(smem + Row::at(e)) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                    continue;
                 }
                 float* const to_p = g.slot_p + slot * g.E + e;
                 int* const to_routes = g.slot_routes + slot * g.E + e;
@@ -679,22 +742,59 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
             if (threadIdx.x == 0) {
                 SlotHead h{0.0f, 0, s_routes, 0};
                 for (int w = 0; w < kWarps; ++w) { h.z += s_z[w]; h.rows += s_rows[w]; }
-                g.head[slot] = h;
+                if (g.one_launch) { s_z[0] = h.z; s_rows[0] = h.rows; } else g.head[slot] = h;
             }
             __syncthreads();
+            summed = true;
             ++s;
         }
         pos = end;
     }
     if (!g.one_launch) return;
-    JoinShared<kWarps>& sh = *reinterpret_cast<JoinShared<kWarps>*>(smem);
-    const int parts = g.S * ((g.E + 31) / 32);
-    __syncthreads();
-    cluster_sync_all();                        // every slot is written
-    for (int i = blockIdx.x; i < parts; i += gridDim.x) { __syncthreads(); join_tile<32>(g, i, sh); }
+    // The blocks are one cluster and there is one sequence: every block joins every eighth expert from the blocks' shared memory.
+    if (!summed) {                             // no rows of the sequence here
+        for (int e = threadIdx.x * 4; e < g.E; e += kRowThreads * 4) *reinterpret_cast<float4*>(smem + Row::at(e)) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int e = threadIdx.x; e < g.E; e += kRowThreads) hist[e] = 0;
+        if (threadIdx.x == 0) { s_z[0] = 0.0f; s_rows[0] = 0; s_routes = 0; }
+    }
     __syncthreads();
     cluster_sync_all();
-    if (blockIdx.x == 0) finish(g, parts, sh);
+    const bool one = lane < kCluster;
+    const float z = group_sum<32>(one ? remote_load(&s_z[0], lane) : 0.0f);
+    const int rows = __reduce_add_sync(kAll, one ? remote_load(&s_rows[0], lane) : 0);
+    int routes = one ? remote_load(&s_routes, lane) : 0;
+    if (g.load != nullptr) {
+        routes = 0;
+        for (int i = lane; i < g.E; i += 32) routes += g.load[i];
+    }
+    routes = __reduce_add_sync(kAll, routes);
+    float part = 0.0f;
+    for (int e = blockIdx.x + threadIdx.x * kCluster; e < g.E; e += kRowThreads * kCluster) {
+        float p = 0.0f;
+        int c = 0;
+#pragma unroll
+        for (int b = 0; b < kCluster; ++b) { p += remote_load(smem + Row::at(e), b); c += remote_load(hist + e, b); }
+        g.counts[e] = c;
+        const int used = g.load != nullptr ? g.load[e] : c;
+        const float a = rows > 0 ? expert_share(g.E, used, routes) / static_cast<float>(rows) : 0.0f;
+        g.coef[e] = a;
+        part += a * p;
+    }
+    part = group_sum<32>(part);
+    __syncthreads();
+    if (lane == 0) s_part[warp] = part;
+    __syncthreads();
+    if (warp == 0) {
+        part = group_sum<32>(lane < kWarps ? s_part[lane] : 0.0f);
+        if (lane == 0) remote_store(&s_parts[blockIdx.x], 0, part);
+    }
+    __syncthreads();
+    cluster_sync_all();                        // nobody leaves while its shared memory may be read
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        float balance = 0.0f;
+        for (int b = 0; b < kCluster; ++b) balance += s_parts[b];
+        write_losses(g, balance, z, rows, rows > 0);
+    }
 }
 
 struct BalanceBwdParams {
@@ -715,7 +815,7 @@ struct BalanceBwdParams {
 // gradient is p c: two operations a value once the sums are there.  The gradient of the chosen weights is scattered into a row
 // of shared memory, K values, and picked up by the lanes that hold their experts.
 template <typename T, int kLanes, int V, bool kSigmoid>
-__global__ void __launch_bounds__(kBwdThreads) balance_bwd_kernel(const BalanceBwdParams g) {
+__global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) balance_bwd_kernel(const BalanceBwdParams g) {
     constexpr int kGroups = kBwdThreads / kLanes;
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // routes a lane, at most (topk <= 32 and <= E)
     using Row = SharedRow<kLanes, V>;
@@ -731,7 +831,7 @@ __global__ void __launch_bounds__(kBwdThreads) balance_bwd_kernel(const BalanceB
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     const int lo = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
-    int s = g.offsets == nullptr ? 0 : first_sequence(g.offsets, g.S, lo, g.T), held = -1;
+    int s = first_sequence(g.offsets, g.S, lo, g.T), held = -1;
     float a[V];                                        // gb times the sequence's f / n
 #pragma unroll
     for (int j = 0; j < V; ++j) a[j] = 0.0f;
@@ -889,7 +989,7 @@ __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const Coun
 template <typename T, int kLanes, int V, bool kSigmoid>
 int launch_rows(const BalanceParams& p, cudaStream_t s) {
     const size_t chosen = p.top_in == nullptr ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
-    const size_t smem = std::max((static_cast<size_t>(kSumRows) * SharedRow<kLanes, V>::kFloats + ((p.E + 1) & ~1) + chosen) * 4, sizeof(JoinShared<kWarps>));
+    const size_t smem = (static_cast<size_t>(kSumRows) * SharedRow<kLanes, V>::kFloats + ((p.E + 1) & ~1) + chosen) * 4;
     if (!p.one_launch) return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid>, p.blocks, kRowThreads, smem, s, false, true, p);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kCluster);
@@ -911,7 +1011,7 @@ int launch_rows(const BalanceParams& p, cudaStream_t s) {
 template <typename T, int kLanes, int V, bool kSigmoid>
 int launch_bwd(BalanceBwdParams p, cudaStream_t s) {
     constexpr int kGroups = kBwdThreads / kLanes;
-    const int blocks = std::min((p.T + kGroups - 1) / kGroups, device_sm_count() * 8);
+    const int blocks = std::min((p.T + kGroups - 1) / kGroups, device_sm_count() * bwd_blocks_per_sm(V, kSigmoid) * 2);
     p.rows_per_block = (p.T + blocks - 1) / blocks;
     return launch_kernel(balance_bwd_kernel<T, kLanes, V, kSigmoid>, blocks, kBwdThreads, 0, s, false, true, p);
 }
@@ -938,6 +1038,7 @@ using namespace mok;
 
 extern "C" size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences) {
     if (bad_sizes(num_tokens, num_experts, 1, num_sequences)) return 0;
+    if (in_one_launch(num_tokens, num_experts, num_sequences)) return 0;
     return Scratch(nullptr, row_blocks(num_tokens, num_experts, num_sequences) + num_sequences, num_experts, num_sequences).bytes;
 }
 
@@ -945,7 +1046,7 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
     if (!args) return MOK_ERR_INVALID;
     const mok_router_balance_args& a = *args;
     const int T = a.num_tokens, E = a.num_experts, K = a.topk, S = a.num_sequences;
-    if (!a.logits || !a.losses || !a.counts || !a.coef || !a.scratch || bad_sizes(T, E, K, S)) return MOK_ERR_INVALID;
+    if (!a.logits || !a.losses || !a.counts || !a.coef || bad_sizes(T, E, K, S)) return MOK_ERR_INVALID;
     if (a.top_experts_in ? (a.top_experts_out || a.router_weights) : (!a.top_experts_out || !a.router_weights)) return MOK_ERR_INVALID;
     if (!a.top_experts_in && (K > 32 || K > E)) return MOK_ERR_INVALID;
     if (!a.sequence_offsets && S != 1) return MOK_ERR_INVALID;
@@ -955,7 +1056,7 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
     p.blocks = row_blocks(T, E, S);
     p.one_launch = in_one_launch(T, E, S);
     const Scratch at(a.scratch, p.blocks + S, E, S);
-    if (a.scratch_bytes < at.bytes || reinterpret_cast<uintptr_t>(a.scratch) % 16) return MOK_ERR_INVALID;
+    if (!p.one_launch && (!a.scratch || a.scratch_bytes < at.bytes || reinterpret_cast<uintptr_t>(a.scratch) % 16)) return MOK_ERR_INVALID;
     p.logits = a.logits;
     p.top_in = reinterpret_cast<const long long*>(a.top_experts_in);
     p.top_out = reinterpret_cast<long long*>(a.top_experts_out);

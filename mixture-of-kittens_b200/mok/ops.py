@@ -987,11 +987,11 @@ def _run_balance(logits: Tensor, T: int, E: int, K: int, top_in: int, experts: i
     counts = torch.empty(S, E, dtype=_I32, device=dev)
     coef = torch.empty(S * E + 2, dtype=_F32, device=dev)
     nbytes = _balance_scratch_bytes(T, E, S)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.launch(dev, what, _lib.mok_router_balance, _lib.pack_router_balance(
         logits.data_ptr(), top_in, experts, weights, 0 if token_mask is None else token_mask.data_ptr(),
         0 if sequence_offsets is None else sequence_offsets.data_ptr(), 0 if load is None else load.data_ptr(), losses.data_ptr(),
-        counts.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes, logits.dtype is _BF16, T, E, K, S, sigmoid))
+        counts.data_ptr(), coef.data_ptr(), scratch.data_ptr() if nbytes else 0, nbytes, logits.dtype is _BF16, T, E, K, S, sigmoid))
     return losses, counts, coef
 
 

@@ -138,6 +138,22 @@ def test_losses_of_finished_routes(cuda_device, T, E, K, S, mask, dtype):
     check(cuda_device, logits, K, where, True, experts=experts, load=load)
 
 
+@pytest.mark.parametrize("offsets", [[0, 0], [0, 5], [130, 137], [250, 256], [40, 200], [256, 256], [300, 900], [-7, 1 << 30]])
+@pytest.mark.parametrize("E,K", [(5, 2), (30, 3), (200, 4), (600, 2)])
+def test_one_sequence_inside_a_small_batch(cuda_device, E, K, offsets):
+    """Blocks whose rows all lie outside the sequence add nothing; bounds are cut to the batch."""
+    logits, _ = make(cuda_device, 256, E, K, seed=E)
+    check(cuda_device, logits, K, {"sequence_offsets": torch.tensor(offsets, dtype=torch.int32)}, False)
+
+
+@pytest.mark.parametrize("E", [8, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 512, 513, 1024])
+def test_batches_around_the_sizes_where_the_kernels_change(cuda_device, E):
+    at_once = 16 * (8 if E <= 16 else 4 if E <= 32 else 2 if E <= 64 else 1)
+    for T in (8 * at_once - 1, 16 * at_once, 16 * at_once + 1):
+        logits, where = make(cuda_device, T, E, 3, seed=T, mask=True)
+        check(cuda_device, logits, 3, where, T % 2 == 0)
+
+
 def test_many_rows_and_few_experts(cuda_device):
     logits, where = make(cuda_device, 70001, 8, 2, S=9, mask=True, seed=4)
     check(cuda_device, logits, 2, where, False)

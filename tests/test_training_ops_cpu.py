@@ -116,9 +116,11 @@ def test_c_entries_refuse_bad_arguments():
         L.pack_router_balance(logits, top, out, w, 0, off, 0, p, p, p, scratch, n, 0, T, E, K, S, 0), None)
     assert L.mok_router_balance(None, None) == L.mok_router_balance_bwd(None, None) == -1
     assert balance(logits=0) == balance(T=0) == balance(E=0) == balance(K=0) == balance(K=256) == balance(S=0) == -1
-    assert balance(S=2) == balance(top=0) == balance(out=p, w=p) == balance(w=p) == balance(top=0, out=p) == balance(scratch=0) == -1
+    assert balance(S=2) == balance(top=0) == balance(out=p, w=p) == balance(w=p) == balance(top=0, out=p) == -1
     assert balance(top=0, out=p, w=p, K=9) == balance(top=0, out=p, w=p, E=64, K=33) == -1
-    assert balance(n=64) == balance(scratch=4104) == -1
+    many = dict(T=100000, E=64)
+    assert balance(n=64, **many) == balance(scratch=4104, **many) == balance(scratch=0, **many) == -1
+    assert L.mok_router_balance_scratch_bytes(512, 8, 1) == 0 < L.mok_router_balance_scratch_bytes(100000, 64, 1)
     assert balance(E=1025) == -3 and balance(T=1 << 24, K=200) == -4
     assert L.mok_router_balance_scratch_bytes(0, 8, 1) == 0
     bwd = lambda *, g=p, T=512, E=8, K=2, S=1, top=0, w=0, dw=0, off=0: L.mok_router_balance_bwd(                              # noqa: E731
