@@ -939,7 +939,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) b
     }
 }
 
-constexpr int kCountThreads = 512;
+constexpr int kCountThreads = 512, kCountBins = 8192;
 struct CountParams {
     const void* top;
     int ids_i32;
@@ -947,11 +947,11 @@ struct CountParams {
     const int* offsets;
     int* counts;                   // [S, E], zeroed before a launch of several blocks
     int T, E, K, S, rows_per_block;
+    int bins;                      // in shared memory, E at least
 };
 
-// Each block counts a run of rows in shared memory, sequence by sequence, and adds what it found: integer sums do not
-// depend on their order.  One block alone stores instead, and clears the counts of sequences without rows itself.  Reads T K
-// ids.
+// Each block counts a run of rows in shared memory, as many sequences at a time as the bins hold, and adds what it found:
+// integer sums do not depend on their order.  One block alone has bins for all and stores them.  Reads T K ids.
 __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const CountParams g) {
     extern __shared__ int bins[];
     pdl_wait();
@@ -960,29 +960,42 @@ __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const Coun
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
     const unsigned topk = g.K;
-    for (int s = alone ? 0 : first_sequence(g.offsets, g.S, pos, g.T); s < g.S && (alone || pos < hi); ++s) {
-        const int begin = max(seq_bound(g.offsets, s, g.T), pos), end = min(seq_bound(g.offsets, s + 1, g.T), hi);
-        if (!alone && begin >= hi) break;
-        if (!alone && end <= begin) continue;
-        for (int e = threadIdx.x; e < g.E; e += kCountThreads) bins[e] = 0;
+    int s = alone ? 0 : first_sequence(g.offsets, g.S, pos, g.T);
+    const int last = alone ? g.S : min(first_sequence(g.offsets, g.S, hi - 1, g.T) + 1, g.S);       // behind the run's sequences
+    auto count = [&](size_t at, int* to) {
+        const long long e = g.ids_i32 ? static_cast<const int*>(g.top)[at] : static_cast<const long long*>(g.top)[at];
+        if (e >= 0 && e < g.E) atomicAdd(to + e, 1);
+    };
+    while (s < last) {
+        const int stop = min(last, s + g.bins / g.E);
+        const int begin = max(seq_bound(g.offsets, s, g.T), pos), end = min(seq_bound(g.offsets, stop, g.T), hi);
+        for (int e = threadIdx.x; e < (stop - s) * g.E; e += kCountThreads) bins[e] = 0;
         __syncthreads();
-        if (end > begin) {
+        if (stop - s == 1 && end > begin) {
             const size_t at = static_cast<size_t>(begin) * topk;
             const unsigned n = static_cast<unsigned>(end - begin) * topk;          // a call has fewer than 2^31 routes
 #pragma unroll 4
-            for (unsigned i = threadIdx.x; i < n; i += kCountThreads) {
-                const long long e = g.ids_i32 ? static_cast<const int*>(g.top)[at + i] : static_cast<const long long*>(g.top)[at + i];
-                if (e >= 0 && e < g.E && (g.mask == nullptr || g.mask[begin + i / topk])) atomicAdd(&bins[e], 1);
+            for (unsigned i = threadIdx.x; i < n; i += kCountThreads)
+                if (g.mask == nullptr || g.mask[begin + i / topk]) count(at + i, bins);
+        } else {
+            for (int t = begin + threadIdx.x; t < end; t += kCountThreads) {
+                if (g.mask != nullptr && !g.mask[t]) continue;
+                int lo = s, up = stop;                     // the last sequence that starts at or before the row
+                while (up - lo > 1) { const int mid = (lo + up) >> 1; if (seq_bound(g.offsets, mid, g.T) <= t) lo = mid; else up = mid; }
+                const size_t at = static_cast<size_t>(t) * topk;
+#pragma unroll 4
+                for (unsigned k = 0; k < topk; ++k) count(at + k, bins + (lo - s) * g.E);
             }
-            pos = end;
         }
         __syncthreads();
         int* const out = g.counts + static_cast<size_t>(s) * g.E;
-        for (int e = threadIdx.x; e < g.E; e += kCountThreads) {
+        for (int e = threadIdx.x; e < (stop - s) * g.E; e += kCountThreads) {
             if (alone) out[e] = bins[e];
             else if (bins[e]) atomicAdd(out + e, bins[e]);
         }
         __syncthreads();
+        pos = max(pos, end);
+        s = stop;
     }
 }
 
@@ -1123,12 +1136,14 @@ extern "C" int mok_expert_counts(const void* top_experts, int ids_i32, int num_t
     if (num_experts > 1024) return MOK_ERR_UNSUPPORTED;
     if (too_many_routes(num_tokens, topk)) return MOK_ERR_TOO_LARGE;
     const long long routes = static_cast<long long>(num_tokens) * topk;
-    const bool alone = routes <= 8192 && num_sequences <= 8;
+    // one block, which needs no cleared counts, takes 8192 routes in the time that clearing them takes
+    const long long bins = static_cast<long long>(num_sequences) * num_experts;
+    const bool alone = routes <= 8192 && bins <= kCountBins;
     const int blocks = alone ? 1 : static_cast<int>(std::min<long long>((routes + 4095) / 4096, device_sm_count() * 4));
     CountParams p{top_experts, ids_i32, token_mask, sequence_offsets, counts, num_tokens, num_experts, topk, num_sequences,
-                  (num_tokens + blocks - 1) / blocks};
+                  (num_tokens + blocks - 1) / blocks, static_cast<int>(std::min<long long>(bins, kCountBins))};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof(kSlotOther, s);
     if (!alone) MOK_CUDA_CHECK(cudaMemsetAsync(counts, 0, static_cast<size_t>(num_sequences) * num_experts * 4, s));
-    return launch_kernel(expert_counts_kernel, blocks, kCountThreads, static_cast<size_t>(num_experts) * 4, s, false, alone, p);
+    return launch_kernel(expert_counts_kernel, blocks, kCountThreads, static_cast<size_t>(p.bins) * 4, s, false, alone, p);
 }

@@ -257,7 +257,7 @@ def test_offsets_beyond_32_bits(cuda_device):
 
 @pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
 @pytest.mark.parametrize("T,E,K,S,mask", [(1, 1, 1, 0, False), (513, 4, 2, 0, True), (7777, 256, 8, 40, True), (3000, 1024, 3, 700, False),
-                                          (100, 60, 255, 3, True)])
+                                          (100, 60, 255, 3, True), (962, 16, 8, 61, True), (50, 900, 4, 9, False), (40000, 300, 2, 500, True), (9000, 8, 3, 4000, False)])
 def test_expert_counts(cuda_device, T, E, K, S, mask, dtype):
     from mok import ops
     _, where = make(cuda_device, T, 4, K, S=S, mask=mask, seed=T)
