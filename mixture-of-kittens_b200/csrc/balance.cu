@@ -33,12 +33,9 @@ constexpr int kSumRows = kWarps / 2;           // rows of E sums in shared memor
 // Blocks of the forward pass, all resident at once on 148 SMs: two an SM up to 512 experts, one above (their rows take twice
 // the registers).  Not read from the device: the order of the sums is the same on every GPU.
 constexpr int row_blocks_per_sm(int E) { return E <= 512 ? 2 : 1; }
-
-
 constexpr int kCluster = 8;                    // blocks of a forward pass in one launch
-constexpr unsigned kAll = 0xffffffffu;
-
 constexpr int kMinCols = 8;                    // fewest experts of a join tile
+constexpr unsigned kAll = 0xffffffffu;
 
 struct SlotHead { float z; int rows, routes, pad; };
 
@@ -128,7 +125,7 @@ template <int kLanes>
 __device__ __forceinline__ float group_max(float v) {       // a NaN loses against any number
     if constexpr (kLanes == 32) {
         float m;
-        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
         return m;
     }
 #pragma unroll
@@ -279,8 +276,8 @@ __device__ __forceinline__ int first_sequence(const int* offsets, int S, int row
 }
 
 // Exponentials, logarithms and quotients go through the hardware's approximate base-2 ones, results below 2^-126 flushed to
-// zero: 2^-22 relative and the rounding of the argument, below what the sums over a row round away.  exp(v - m) is
-// 2^(v log2(e) - m log2(e)), one fused multiply-add.
+// zero: 2^-22 relative and the rounding of the argument, below what the sums over a row round away.  The row's maximum is taken
+// off before the multiplication by log2(e): a row of the type's lowest value would overflow in one fused multiply-add.
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float rcp_fast(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -303,10 +300,10 @@ __device__ __forceinline__ RowStats row_stats(const float (&v)[V], float (&ex)[V
 #pragma unroll
     for (int j = 1; j < V; ++j) m = fmaxf(m, v[j]);
     m = group_max<kLanes>(m);
-    const float base = m > -INFINITY ? m : 0.0f, shift = -base * kLog2e;
+    const float base = m > -INFINITY ? m : 0.0f;
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) { ex[j] = exp2_fast(fmaf(v[j], kLog2e, shift)); sum += ex[j]; }     // lanes past E hold -inf: 0
+    for (int j = 0; j < V; ++j) { ex[j] = exp2_fast((v[j] - base) * kLog2e); sum += ex[j]; }     // lanes past E hold -inf: 0
     sum = group_sum<kLanes>(sum);
     RowStats r;
     r.inv = sum == 0.0f ? 0.0f : rcp_fast(sum);
@@ -380,7 +377,7 @@ __device__ __forceinline__ void select_in_rounds(const float (&v)[V], int E, int
 
 __device__ __forceinline__ float warp_min(float v) {
     float m;
-    asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
     return m;
 }
 
@@ -404,8 +401,8 @@ __device__ __forceinline__ int gather_above(const float (&v)[V], float t, uint2*
 
 // One row a warp.  Let the lanes form K sets of `set` neighbours, as large as they can be, and t be the least of the sets'
 // maxima: at least K values are >= t, and few more.  They are gathered, one a lane, and every lane counts those that come
-// before its own.  Where more than 32 are >= t (with K = 8 of 256 in 8 rows of 100), t is the K-th largest of the lanes' maxima instead, and
-// where that does not do either (many equal values, few above -inf, no such sets: set = 0) the row goes in rounds.
+// before its own.  Where more than 32 are >= t (with K = 8 of 256 in 8 rows of 100), t is the K-th largest of the lanes' maxima
+// instead, and where that does not do either (many equal values, few above -inf, no such sets: set = 0) the row goes in rounds.
 template <int V>
 __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K, int set, uint2* gathered, float2* chosen) {
     const int lane = threadIdx.x & 31;
@@ -561,9 +558,7 @@ __device__ __forceinline__ void finish(const BalanceParams& g, int parts, JoinSh
         z = group_sum<32>(one ? sh.z[lane] : 0.0f);
         rows = warp_sum(one ? sh.rows[lane] : 0);
         live = warp_sum(one ? sh.routes[lane] : 0);
-        if (lane == 0) {
-            write_losses(g, balance, z, rows, live);
-        }
+        if (lane == 0) write_losses(g, balance, z, rows, live);
     }
 }
 
@@ -718,7 +713,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
             if (lane == 0) { s_z[warp] = z; s_rows[warp] = rows; }
             __syncthreads();
             const size_t slot = static_cast<size_t>(blockIdx.x) + s;
-            for (int e = threadIdx.x * 4; e < g.E; e += kRowThreads * 4) {     // (once: a block has at least 256 threads)
+            for (int e = threadIdx.x * 4; e < g.E; e += kRowThreads * 4) {
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int w = 0; w < kSumRows; ++w) {

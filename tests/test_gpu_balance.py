@@ -178,6 +178,35 @@ def test_empty_rows_and_masked_experts(cuda_device):
     assert torch.isfinite(ops.router_balance_bwd(torch.ones(2, device=cuda_device), low, coef)).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E", [6, 60, 300])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_rows_of_the_lowest_value(cuda_device, E, dtype, sigmoid):
+    """A row whose every logit is the type's lowest value is uniform, not empty; lse^2 overflows, so no z-loss is asked for."""
+    from mok import ops
+    T, K = 40, 4
+    logits = make(cuda_device, T, E, K, dtype=dtype, seed=E)[0]
+    logits[7:12] = torch.finfo(dtype).min
+    logits[20, 3:] = torch.finfo(dtype).min
+    x = logits.to(cuda_device)
+    experts, weights, losses, counts, coef = ops.router_topk_balance(x, K, sigmoid=sigmoid)
+    chosen = O.select(logits.float().numpy(), K)
+    assert np.array_equal(experts.cpu().numpy(), chosen) and float(weights[7:12].sub(1 / K).abs().max()) < WEIGHT
+    l64 = logits.double().requires_grad_(True)
+    uniform = torch.zeros(T, E, dtype=torch.float64)        # the 64-bit oracle on rows shifted to zero: the same probabilities
+    uniform[7:12] = -torch.finfo(dtype).min
+    ref = O.losses(l64 + uniform if not sigmoid else torch.where(uniform != 0, l64 * 0, l64), chosen, sigmoid=sigmoid)[0]
+    assert abs(float(losses[0]) - float(ref)) <= LOSS * float(ref)
+    got = ops.router_balance_bwd(torch.tensor([1.0, 0.0], device=cuda_device), x, coef, None, None, experts, weights,
+                                 torch.ones_like(weights), sigmoid)
+    assert bool(torch.isfinite(got).all())
+    if not sigmoid:
+        grad, = torch.autograd.grad(ref, l64)
+        a = O.expert_counts(chosen, E) * E / counts.sum().item() / T
+        scale = 2 * torch.from_numpy(a).max() + 2.0 ** -20       # weights of a row add up to 1 within WEIGHT
+        assert float((got.cpu().double() - grad).abs().max()) <= (GRAD + (2.0 ** -8 if dtype == torch.bfloat16 else 0)) * float(scale) + WEIGHT
+
+
 def test_far_below_zero_sigmoids_do_not_vanish(cuda_device):
     logits = torch.randn(200, 16, generator=torch.Generator().manual_seed(2)) * 3 - 150.0       # sigma underflows in f32
     check(cuda_device, logits, 3, {}, True)
