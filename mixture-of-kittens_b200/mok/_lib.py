@@ -205,10 +205,12 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 def launch(device: torch.device, what: str, entry, *args) -> None:
     """Calls `entry(*args, stream)` with `device` current, whatever device the caller has made current."""
     if device.index is None or device.index == _current_device():
-        check(entry(*args, stream_ptr(device)), what)
+        rc = entry(*args, stream_ptr(device))
     else:
         with torch.cuda.device(device):
-            check(entry(*args, stream_ptr(device)), what)
+            rc = entry(*args, stream_ptr(device))
+    if rc:
+        check(rc, what)
 
 
 def ptr_array(ptrs) -> C.Array:

@@ -1039,27 +1039,27 @@ def router_balance_bwd(d_losses: Tensor, logits: Tensor, coef: Tensor, token_mas
     T, E = _balance_logits(logits)
     dev = logits.device
     S = 1 if token_mask is None and sequence_offsets is None else _sequences(T, dev, token_mask, sequence_offsets)
-    for t, n in ((d_losses, 2), (coef, S * E + 2)):
-        if not (t.shape == (n,) and t.device == dev and t.is_contiguous()):
-            raise ValueError("d_losses must be contiguous [2] and coef [num_sequences * num_experts + 2], on the device of the logits")
-        if t.dtype is not _F32:
-            raise TypeError("d_losses and coef must have dtype torch.float32")
+    if d_losses.dtype is not _F32 or coef.dtype is not _F32:
+        raise TypeError("d_losses and coef must have dtype torch.float32")
+    if not (d_losses.shape == (2,) and d_losses.is_contiguous() and d_losses.device == dev
+            and coef.shape == (S * E + 2,) and coef.is_contiguous() and coef.device == dev):
+        raise ValueError("d_losses must be contiguous [2] and coef [num_sequences * num_experts + 2], on the device of the logits")
     if type(sigmoid) is not bool:
         raise TypeError("sigmoid must be a boolean")
-    if (top_experts is None) != (router_weights is None) or (top_experts is None) != (d_router_weights is None):
-        raise ValueError("top_experts, router_weights and d_router_weights come together or not at all")
     K = 1
     top = w = d_w = 0
-    if top_experts is not None:
+    if top_experts is not None and router_weights is not None and d_router_weights is not None:
         T_routes, K = _routes(top_experts)
         if T_routes != T or K > min(32, E) or top_experts.device != dev:
             raise ValueError("top_experts must be [num_tokens, topk] with topk <= min(32, num_experts), on the device of the logits")
-        for t in (router_weights, d_router_weights):
-            if not (t.shape == (T, K) and t.device == dev and t.is_contiguous()):
-                raise ValueError("router_weights and d_router_weights must be contiguous and match top_experts")
-            if t.dtype is not _F32:
-                raise TypeError("router_weights and d_router_weights must have dtype torch.float32")
+        if router_weights.dtype is not _F32 or d_router_weights.dtype is not _F32:
+            raise TypeError("router_weights and d_router_weights must have dtype torch.float32")
+        if not (router_weights.shape == d_router_weights.shape == (T, K) and router_weights.is_contiguous()
+                and d_router_weights.is_contiguous() and router_weights.device == dev and d_router_weights.device == dev):
+            raise ValueError("router_weights and d_router_weights must be contiguous and match top_experts")
         top, w, d_w = top_experts.data_ptr(), router_weights.data_ptr(), d_router_weights.data_ptr()
+    elif not (top_experts is None and router_weights is None and d_router_weights is None):
+        raise ValueError("top_experts, router_weights and d_router_weights come together or not at all")
     d_logits = torch.empty_like(logits)
     if T > 0:
         _lib.launch(dev, "router_balance_bwd", _lib.mok_router_balance_bwd, _lib.pack_router_balance_bwd(

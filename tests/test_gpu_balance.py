@@ -474,3 +474,49 @@ def test_two_captured_graphs_share_nothing(cuda_device):
     torch.cuda.synchronize()
     for a, b in zip(want, got):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_compiled_and_threaded_calls(cuda_device):
+    """Traced whole by torch.compile, and called by several host threads at once on streams of their own."""
+    import threading
+    from mok import functional as F, ops
+    logits, where = make(cuda_device, 700, 48, 3, S=4, mask=True, seed=21)
+    where = on(cuda_device, where)
+    x = logits.to(cuda_device)
+    off, mask = where["sequence_offsets"], where["token_mask"]
+
+    def step(l, r, seed):
+        experts, weights, losses, counts, coef = ops.router_topk_balance(l, 3, mask, off)
+        d = ops.router_balance_bwd(losses, l, coef, mask, off, experts, weights, weights)
+        return experts, weights, losses, counts, d, ops.expert_counts(experts, 48), ops.dropout_add(r, r, seed, 0.3), ops.dropout_add_bwd(r, seed, 0.3)
+    r = torch.randn(100, 64, device=cuda_device)
+    seed = torch.tensor([5], device=cuda_device)
+    want = step(x, r, seed)
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(x, r, seed)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+    leaf = x.clone().requires_grad_(True)
+
+    def loss(l):
+        _, weights, bal = F.route_balanced(l, 3, **where)
+        return (weights * weights).sum() + bal.losses.sum()
+    grad, = torch.autograd.grad(loss(leaf), leaf)
+    grad_c, = torch.autograd.grad(torch.compile(loss, backend="aot_eager")(leaf), leaf)
+    assert torch.equal(grad, grad_c)
+
+    failed = []
+
+    def work():
+        try:
+            stream = torch.cuda.Stream(cuda_device)
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    if not all(torch.equal(a, b) for a, b in zip(want, step(x, r, seed))):
+                        raise AssertionError("other bytes")
+        except Exception as e:                              # noqa: BLE001 - reported below
+            failed.append(e)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed, failed
