@@ -180,15 +180,28 @@ template <int n> __device__ __forceinline__ void store_chunk(__nv_bfloat16* p, c
     else *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
 }
 
-// A row of E values: the group's lane l holds values l V .. l V + V - 1 (so the lowest expert among equals is the lowest lane's
-// first).  Values past E read as `fill`.
-template <int V, typename T>
-__device__ __forceinline__ void load_row(const T* row, int e0, int E, int chunk, float fill, float (&v)[V]) {
+// How a group of kLanes lanes holds a row of E values, V a lane: eight (four, where V is four) neighbours a lane at a time, so
+// that the group's accesses are contiguous.  A lane's values are in the order of the experts.
+template <int kLanes, int V> struct Held {
+    static constexpr int kUnit = V < 8 ? V : 8;
+    static __device__ __forceinline__ int expert(int l, int j) { return (j / kUnit) * (kLanes * kUnit) + l * kUnit + j % kUnit; }
+    static __device__ __forceinline__ int count(int l, int E) {          // values of lane l that are there
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < V; j += kUnit) n += min(max(E - expert(l, j), 0), kUnit);
+        return n;
+    }
+};
+
+// Values past E read as `fill`.
+template <int kLanes, int V, typename T>
+__device__ __forceinline__ void load_row(const T* row, int l, int E, int chunk, float fill, float (&v)[V]) {
+    using At = Held<kLanes, V>;
     if constexpr (V >= 8) {
         if (chunk == 8) {
 #pragma unroll
             for (int j = 0; j < V; j += 8) {
-                if (e0 + j < E) load_chunk<8>(row + e0 + j, v + j);
+                if (At::expert(l, j) < E) load_chunk<8>(row + At::expert(l, j), v + j);
                 else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[j + i] = fill;
@@ -200,29 +213,30 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, int chunk,
     if (chunk >= 4) {
 #pragma unroll
         for (int j = 0; j < V; j += 4) {
-            if (e0 + j < E) load_chunk<4>(row + e0 + j, v + j);
+            if (At::expert(l, j) < E) load_chunk<4>(row + At::expert(l, j), v + j);
             else { v[j] = fill; v[j + 1] = fill; v[j + 2] = fill; v[j + 3] = fill; }
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = e0 + j < E ? to_float(row[e0 + j]) : fill;
+        for (int j = 0; j < V; ++j) v[j] = At::expert(l, j) < E ? to_float(row[At::expert(l, j)]) : fill;
     }
 }
-template <int V, typename T>
-__device__ __forceinline__ void store_row(T* row, int e0, int E, int chunk, const float (&v)[V]) {
+template <int kLanes, int V, typename T>
+__device__ __forceinline__ void store_row(T* row, int l, int E, int chunk, const float (&v)[V]) {
+    using At = Held<kLanes, V>;
     if constexpr (V >= 8) {
         if (chunk == 8) {
 #pragma unroll
-            for (int j = 0; j < V; j += 8) if (e0 + j < E) store_chunk<8>(row + e0 + j, v + j);
+            for (int j = 0; j < V; j += 8) if (At::expert(l, j) < E) store_chunk<8>(row + At::expert(l, j), v + j);
             return;
         }
     }
     if (chunk >= 4) {
 #pragma unroll
-        for (int j = 0; j < V; j += 4) if (e0 + j < E) store_chunk<4>(row + e0 + j, v + j);
+        for (int j = 0; j < V; j += 4) if (At::expert(l, j) < E) store_chunk<4>(row + At::expert(l, j), v + j);
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) if (e0 + j < E) from_float(v[j], row[e0 + j]);
+        for (int j = 0; j < V; ++j) if (At::expert(l, j) < E) from_float(v[j], row[At::expert(l, j)]);
     }
 }
 
@@ -251,7 +265,10 @@ __device__ __forceinline__ void remote_store(float* p, int block, float v) {
 template <int kLanes, int V> struct SharedRow {
     static constexpr int kFloats = V * (kLanes + 1);
     static __device__ __forceinline__ int chunk(int lane, int j) { return ((j >> 2) * (kLanes + 1) + lane) << 2; }
-    static __device__ __forceinline__ int at(int e) { return chunk(e / V, e % V) + (e & 3); }
+    static __device__ __forceinline__ int at(int e) {
+        constexpr int kUnit = Held<kLanes, V>::kUnit;
+        return chunk(e / kUnit % kLanes, e / (kLanes * kUnit) * kUnit + e % kUnit) + (e & 3);
+    }
 };
 
 // Sequence bounds as the kernels use them: inside [0, T] whatever the caller's array holds.
@@ -347,7 +364,8 @@ __device__ __forceinline__ void select_in_rounds(const float (&v)[V], int E, int
     const int lane = threadIdx.x & 31, l = lane % kLanes;
     const unsigned group = kLanes == 32 ? kAll : ((1u << kLanes) - 1u) << (lane - l);
     const unsigned below = (1u << lane) - 1u;
-    const int mine = min(max(E - l * V, 0), V);                   // values of this lane that are there
+    using At = Held<kLanes, V>;
+    const int mine = At::count(l, E);
     unsigned taken = 0;
     float b1, b2;
     int j1, j2;
@@ -356,8 +374,12 @@ __device__ __forceinline__ void select_in_rounds(const float (&v)[V], int E, int
         const float best = group_max<kLanes>(b1);
         const bool equal = j1 < V && b1 == best;
         const unsigned at = __ballot_sync(kAll, equal) & group;
-        const bool win = equal && (at & below) == 0;
-        if (win) chosen[k] = make_float2(best, __int_as_float(l * V + j1));
+        bool win = equal && (at & below) == 0;
+        if (V > At::kUnit && __any_sync(kAll, (at & (at - 1)) != 0)) {          // equals in several lanes, whose experts interleave
+            const int e = equal ? At::expert(l, j1) : 0x7fffffff;
+            win = e == group_min<kLanes>(e) && equal;
+        }
+        if (win) chosen[k] = make_float2(best, __int_as_float(At::expert(l, j1)));
         taken |= win ? 1u << (j1 & 31) : 0u;
         const bool dry = win && j2 == V;
         b1 = win ? b2 : b1;
@@ -366,7 +388,7 @@ __device__ __forceinline__ void select_in_rounds(const float (&v)[V], int E, int
         j2 = win ? V : j2;
         if (__any_sync(kAll, at == 0)) {                           // nothing above -inf left: the lowest experts not taken yet
             const unsigned left = ~taken & (V == 32 && mine == 32 ? kAll : (1u << mine) - 1u);
-            const int e = left ? l * V + __ffs(left) - 1 : 0x7fffffff;
+            const int e = left ? At::expert(l, __ffs(left) - 1) : 0x7fffffff;
             const int lowest = group_min<kLanes>(e);
             if (at == 0 && e == lowest && left) { chosen[k] = make_float2(-INFINITY, __int_as_float(e)); taken |= left & (0u - left); }
         }
@@ -392,7 +414,7 @@ __device__ __forceinline__ int gather_above(const float (&v)[V], float t, uint2*
         const bool in = v[j] >= t;
         const unsigned at = __ballot_sync(kAll, in);
         if (V <= 8 || at != 0) {
-            if (in) gathered[(n + __popc(at & below)) & 31] = make_uint2(lane * V + j, __float_as_uint(v[j]));
+            if (in) gathered[(n + __popc(at & below)) & 31] = make_uint2(Held<32, V>::expert(lane, j), __float_as_uint(v[j]));
             n += __popc(at);
         }
     }
@@ -597,12 +619,13 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
     int* const hist = reinterpret_cast<int*>(smem + kSumRows * Row::kFloats);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes;
     float2* const chosen = reinterpret_cast<float2*>(hist + ((g.E + 1) & ~1)) + static_cast<size_t>(group) * g.K;
-    const int e0 = l * V;
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0 && !g.one_launch) *g.ticket = 0;
     const bool select = g.top_in == nullptr;
-    int set = 32;                                              // select_by_rank: the largest sets of lanes of which there are K
-    while (set > 0 && (g.E + set * V / 2) / (set * V) < g.K) set >>= 1;         // (one that is half full counts)
+    // select_by_rank: the largest sets of lanes of which there are K (one of which half the lanes have values counts)
+    const int lanes = min(32, (g.E + Held<kLanes, V>::kUnit - 1) / Held<kLanes, V>::kUnit);
+    int set = 32;
+    while (set > 0 && (lanes + set / 2) / set < g.K) set >>= 1;
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
@@ -625,7 +648,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
         for (int j = 0; j < V; ++j) acc[j] = 0.0f;
         // all lanes of a warp stay in step; groups past the run work on nothing
         auto load = [&](int t0, float (&v)[V]) {
-            load_row<V>(static_cast<const T*>(g.logits) + static_cast<size_t>(min(t0 + lane / kLanes, end - 1)) * g.E, e0, g.E, g.chunk, -INFINITY, v);
+            load_row<kLanes, V>(static_cast<const T*>(g.logits) + static_cast<size_t>(min(t0 + lane / kLanes, end - 1)) * g.E, l, g.E, g.chunk, -INFINITY, v);
         };
         float next[V];
         const int t_first = pos + warp * (32 / kLanes);
@@ -815,7 +838,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) b
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // routes a lane, at most (topk <= 32 and <= E)
     using Row = SharedRow<kLanes, V>;
     __shared__ alignas(16) float s_add[kGroups][Row::kFloats];
-    const int lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes, e0 = l * V;
+    const int lane = threadIdx.x & 31, l = lane % kLanes, group = threadIdx.x / kLanes;
     float* const add = s_add[group];
 #pragma unroll
     for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(add + Row::chunk(l, j)) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -836,7 +859,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) b
         const bool there = t < hi;
         const T* const row = static_cast<const T*>(g.logits) + static_cast<size_t>(there ? t : t0) * g.E;
         float d[V], v[V];
-        if (losses) load_row<V>(row, e0, g.E, g.chunk, -INFINITY, v);
+        if (losses) load_row<kLanes, V>(row, l, g.E, g.chunk, -INFINITY, v);
         int expert[kPer];
         float w[kPer], dw[kPer];
         if (g.top != nullptr) {
@@ -856,7 +879,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) b
             live = live && s < g.S && seq_bound(g.offsets, s, g.T) <= t;
         }
         if (live && s != held) {
-            load_row<V>(g.coef + static_cast<size_t>(s) * g.E, e0, g.E, g.coef_chunk, 0.0f, a);
+            load_row<kLanes, V>(g.coef + static_cast<size_t>(s) * g.E, l, g.E, g.coef_chunk, 0.0f, a);
 #pragma unroll
             for (int j = 0; j < V; ++j) a[j] *= gb;
             held = s;
@@ -930,7 +953,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) b
             for (int i = 0; i < kPer; ++i) if (expert[i] >= 0) add[expert[i]] = 0.0f;
             __syncwarp();
         }
-        if (there) store_row<V>(static_cast<T*>(g.d_logits) + static_cast<size_t>(t) * g.E, e0, g.E, g.chunk, d);
+        if (there) store_row<kLanes, V>(static_cast<T*>(g.d_logits) + static_cast<size_t>(t) * g.E, l, g.E, g.chunk, d);
     }
 }
 
