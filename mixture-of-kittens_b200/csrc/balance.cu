@@ -602,18 +602,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) balance_join_kernel(const Bal
 }
 
 // Bound by instructions and, without the choice, by the latency of its loads.  Reads T E logits once, writes K routes a row and (p,
-// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 79 (21), finished routes
-// 44; 65536 x 500 bf16, K = 6, 61 sequences: 70 (10) and 43; 16384 x 128: 16 (1.3) and 11.  A row of 256 takes 500 instructions
+// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 78 (21), finished routes
+// 36; 65536 x 500 bf16, K = 6, 61 sequences: 69 (10) and 32; 16384 x 128: 16 (1.3) and 10.  A row of 256 takes 500 instructions
 // with the choice, 180 without; in rounds of one maximum each the choice alone took 540.  Loading the next row ahead: 53 -> 44
-// without the choice at 256 experts; above, the registers it takes cost a block an SM (44 -> 59 at 500).
-template <typename T, int kLanes, int V, bool kSigmoid>
+// without the choice at 256 experts; above, the registers it takes cost more (36 -> 46 at 500).  Finished routes are counted for a
+// run's rows at once; with their row, each row waited for its ids (44 -> 36).  Rows staged in shared memory two to four ahead by
+// asynchronous copies were slower throughout (44 -> 55, backward 54 -> 73 to 77).
+template <typename T, int kLanes, int V, bool kSigmoid, bool kSelect>
 __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) balance_rows_kernel(const BalanceParams g) {
     using Row = SharedRow<kLanes, V>;
     constexpr bool kAhead = V <= 8;            // the next row is loaded while this one is worked on
     constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // chosen experts a lane, at most (K <= 32 and <= E)
     extern __shared__ __align__(16) float smem[];               // sums of p [kSumRows], routes [E], then the chosen (value, expert) [kGroups][K]
-    __shared__ alignas(16) uint2 s_gathered[kLanes == 32 ? kWarps : 1][32];
+    __shared__ alignas(16) uint2 s_gathered[kSelect && kLanes == 32 ? kWarps : 1][32];
     __shared__ float s_z[kWarps], s_part[kWarps], s_parts[kCluster];
     __shared__ int s_rows[kWarps], s_routes;
     int* const hist = reinterpret_cast<int*>(smem + kSumRows * Row::kFloats);
@@ -621,7 +623,6 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
     float2* const chosen = reinterpret_cast<float2*>(hist + ((g.E + 1) & ~1)) + static_cast<size_t>(group) * g.K;
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0 && !g.one_launch) *g.ticket = 0;
-    const bool select = g.top_in == nullptr;
     // select_by_rank: the largest sets of lanes of which there are K (one of which half the lanes have values counts)
     const int lanes = min(32, (g.E + Held<kLanes, V>::kUnit - 1) / Held<kLanes, V>::kUnit);
     int set = 32;
@@ -646,14 +647,23 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
         int rows = 0, routes = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+        if (!kSelect && counted) {             // finished routes, of all the run's rows at once
+            const size_t at = static_cast<size_t>(pos) * g.K;
+            const unsigned n = static_cast<unsigned>(end - pos) * static_cast<unsigned>(g.K);        // a call has fewer than 2^31 routes
+#pragma unroll 4
+            for (unsigned i = threadIdx.x; i < n; i += kRowThreads) {
+                const long long e = g.top_in[at + i];
+                if (e >= 0 && e < g.E && (g.mask == nullptr || g.mask[pos + i / static_cast<unsigned>(g.K)])) { atomicAdd(&hist[e], 1); ++routes; }
+            }
+        }
         // all lanes of a warp stay in step; groups past the run work on nothing
         auto load = [&](int t0, float (&v)[V]) {
             load_row<kLanes, V>(static_cast<const T*>(g.logits) + static_cast<size_t>(min(t0 + lane / kLanes, end - 1)) * g.E, l, g.E, g.chunk, -INFINITY, v);
         };
         float next[V];
         const int t_first = pos + warp * (32 / kLanes);
-        if (kAhead && t_first < end && (counted || select)) load(t_first, next);
-        for (int t0 = t_first; t0 < end && (counted || select); t0 += kGroups) {
+        if (kAhead && t_first < end && (counted || kSelect)) load(t_first, next);
+        for (int t0 = t_first; t0 < end && (counted || kSelect); t0 += kGroups) {
             const int t = t0 + lane / kLanes;
             const bool there = t < end;
             float v[V];
@@ -665,8 +675,8 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
                 load(t0, v);
             }
             const bool live = there && counted && (g.mask == nullptr || g.mask[t]);
-            const size_t o = static_cast<size_t>(t) * g.K;
-            if (select) {
+            if constexpr (kSelect) {
+                const size_t o = static_cast<size_t>(t) * g.K;
                 if constexpr (kLanes == 32) select_by_rank<V>(v, g.E, g.K, set, s_gathered[warp], chosen);
                 else select_in_rounds<kLanes, V>(v, g.E, g.K, chosen);
                 const float top = chosen[0].x;
@@ -694,11 +704,6 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
                     }
                 }
                 __syncwarp();
-            } else if (live) {
-                for (int k = l; k < g.K; k += kLanes) {
-                    const long long e = g.top_in[o + k];
-                    if (e >= 0 && e < g.E) { atomicAdd(&hist[e], 1); ++routes; }
-                }
             }
             if (counted) {
                 float ex[V], sg[V];
@@ -1017,11 +1022,11 @@ __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const Coun
     }
 }
 
-template <typename T, int kLanes, int V, bool kSigmoid>
+template <typename T, int kLanes, int V, bool kSigmoid, bool kSelect>
 int launch_rows(const BalanceParams& p, cudaStream_t s) {
-    const size_t chosen = p.top_in == nullptr ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
+    const size_t chosen = kSelect ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
     const size_t smem = (static_cast<size_t>(kSumRows) * SharedRow<kLanes, V>::kFloats + ((p.E + 1) & ~1) + chosen) * 4;
-    if (!p.one_launch) return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid>, p.blocks, kRowThreads, smem, s, false, true, p);
+    if (!p.one_launch) return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid, kSelect>, p.blocks, kRowThreads, smem, s, false, true, p);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kCluster);
     cfg.blockDim = dim3(kRowThreads);
@@ -1034,9 +1039,15 @@ int launch_rows(const BalanceParams& p, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    auto* kern = balance_rows_kernel<T, kLanes, V, kSigmoid>;
+    auto* kern = balance_rows_kernel<T, kLanes, V, kSigmoid, kSelect>;
     MOK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
     return MOK_OK;
+}
+
+template <typename T, int kLanes, int V>
+int launch_rows_as(const BalanceParams& p, cudaStream_t s) {
+    if (p.top_in == nullptr) return p.sigmoid ? launch_rows<T, kLanes, V, true, true>(p, s) : launch_rows<T, kLanes, V, false, true>(p, s);
+    return p.sigmoid ? launch_rows<T, kLanes, V, true, false>(p, s) : launch_rows<T, kLanes, V, false, false>(p, s);
 }
 
 template <typename T, int kLanes, int V, bool kSigmoid>
@@ -1108,11 +1119,11 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
     ProfScope prof(kSlotOther, s, p.one_launch ? 1 : 2);
     int rc;
     if (a.logits_bf16) {
-#define MOK_CALL(lanes, v) (p.sigmoid ? launch_rows<__nv_bfloat16, lanes, v, true>(p, s) : launch_rows<__nv_bfloat16, lanes, v, false>(p, s))
+#define MOK_CALL(lanes, v) launch_rows_as<__nv_bfloat16, lanes, v>(p, s)
         rc = MOK_ROW_SHAPE(E, MOK_CALL);
 #undef MOK_CALL
     } else {
-#define MOK_CALL(lanes, v) (p.sigmoid ? launch_rows<float, lanes, v, true>(p, s) : launch_rows<float, lanes, v, false>(p, s))
+#define MOK_CALL(lanes, v) launch_rows_as<float, lanes, v>(p, s)
         rc = MOK_ROW_SHAPE(E, MOK_CALL);
 #undef MOK_CALL
     }
