@@ -169,7 +169,8 @@ int mok_router_topk_bwd(const int32_t* top_experts_i32, const float* router_weig
  * Either top_experts_in int64 [T, K] holds finished routes (ids outside [0, E) go nowhere, topk <= 255) and the next two are
  * NULL, or it is NULL and the call also chooses the K largest logits of every row (topk <= 32; descending, lower expert
  * first among equals) into top_experts_out int64 and router_weights f32 [T, K] (softmax, or sigmas over their sum, of those K).
- * load: int32 [num_sequences, E] that stands for the counts in f (NULL: the counts).  Outputs: losses f32 [2], counts int32
+ * num_tokens * topk stays below 2^31 - 2^16.
+ * load: int32 [num_sequences, E] that stands for the counts in f, a sequence's sum below 2^31 (NULL: the counts).  Outputs: losses f32 [2], counts int32
  * [num_sequences, E], coef f32 [num_sequences * E + 2] for mok_router_balance_bwd.  scratch: 16-byte aligned,
  * mok_router_balance_scratch_bytes bytes (0: none is needed, NULL will do), of this call alone until it has run.
  * mok_router_balance_bwd writes all of d_logits (type of logits) from d_losses f32 [2] and, where the three are not NULL,

@@ -1071,7 +1071,8 @@ int launch_bwd(BalanceBwdParams p, cudaStream_t s) {
     }()
 
 bool bad_sizes(int T, int E, int K, int S) { return T <= 0 || E <= 0 || K <= 0 || K > 255 || S <= 0; }
-bool too_many_routes(int T, int K) { return static_cast<long long>(T) * K > 0x7fffffffll; }      // counts are 32-bit
+// counts are 32-bit, and a row index and a block's rows have to fit an int together
+bool too_many_routes(int T, int K) { return T > 0x7fff0000 || static_cast<long long>(T) * K > 0x7fffffffll; }
 
 }  // namespace
 }  // namespace mok
@@ -1142,7 +1143,7 @@ extern "C" int mok_router_balance_bwd(const mok_router_balance_bwd_args* args, v
     if (with != 0 && (with != 3 || K > 32 || K > E)) return MOK_ERR_INVALID;
     if (!a.sequence_offsets && S != 1) return MOK_ERR_INVALID;
     if (E > 1024) return MOK_ERR_UNSUPPORTED;
-    if (static_cast<long long>(S) * E > 0x7fffffffll) return MOK_ERR_TOO_LARGE;
+    if (T > 0x7fff0000 || static_cast<long long>(S) * E > 0x7fffffffll) return MOK_ERR_TOO_LARGE;
     BalanceBwdParams p{a.d_losses, a.logits, a.coef, a.token_mask, a.sequence_offsets, reinterpret_cast<const long long*>(a.top_experts),
                        a.router_weights, a.d_router_weights, a.d_logits, T, E, K, S, a.sigmoid, 0,
                        std::min(chunk_of(a.logits, E, bytes), chunk_of(a.d_logits, E, bytes)), chunk_of(a.coef, E, 4)};

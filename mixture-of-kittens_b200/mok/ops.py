@@ -931,6 +931,7 @@ torch.library.register_autograd("mok::router_topk", _router_backward, setup_cont
 # ------------------------------------------------------------------------------------------
 # losses that keep the experts evenly used, and the counts behind them (no reference op)
 # ------------------------------------------------------------------------------------------
+_MOST_TOKENS = (1 << 31) - (1 << 16)
 _F32, _BF16, _I32, _I64, _BOOL = torch.float32, torch.bfloat16, torch.int32, torch.int64, torch.bool
 
 
@@ -955,6 +956,8 @@ def _balance_logits(logits: Tensor) -> tuple[int, int]:
     T, E = logits.shape
     if not 0 < E <= 1024:
         raise ValueError("num_experts must be in [1, 1024]")
+    if T > _MOST_TOKENS:
+        raise ValueError("num_tokens exceeds this build's limit of 2^31 - 2^16")
     return T, E
 
 
@@ -966,6 +969,8 @@ def _routes(top_experts: Tensor, dtypes=(_I64,)) -> tuple[int, int]:
     T, K = top_experts.shape
     if not 0 < K <= 255:
         raise ValueError("topk must be in [1, 255]")
+    if T * K > _MOST_TOKENS:
+        raise ValueError("num_tokens * topk exceeds this build's limit of 2^31 - 2^16")
     return T, K
 
 
@@ -1004,8 +1009,8 @@ def router_balance(logits: Tensor, top_experts: Tensor, token_mask: Tensor | Non
     over the tokens that count: balance is sum_e f_e P_e, averaged over the sequences that hold a token that counts (1 when
     everything is even); z is the mean of logsumexp(logits)^2.  A token counts if `token_mask` (bool [T]) is set and it lies in
     [sequence_offsets[0], sequence_offsets[-1]) (int32, not decreasing; None: one sequence of all tokens).  Ids outside
-    [0, E) are routes that go nowhere.  `load` (int32, the shape of counts) stands for the local counts in f: counts that
-    ranks have added up.  Differentiable with respect to the logits."""
+    [0, E) are routes that go nowhere.  `load` (int32, the shape of counts, a sequence's sum below 2^31) stands for the local
+    counts in f: counts that ranks have added up.  Differentiable with respect to the logits."""
     T, E = _balance_logits(logits)
     T_routes, K = _routes(top_experts)
     if T_routes != T or top_experts.device != logits.device:

@@ -121,13 +121,13 @@ def test_c_entries_refuse_bad_arguments():
     many = dict(T=100000, E=64)
     assert balance(n=64, **many) == balance(scratch=4104, **many) == balance(scratch=0, **many) == -1
     assert L.mok_router_balance_scratch_bytes(512, 8, 1) == 0 < L.mok_router_balance_scratch_bytes(100000, 64, 1)
-    assert balance(E=1025) == -3 and balance(T=1 << 24, K=200) == -4
+    assert balance(E=1025) == -3 and balance(T=1 << 24, K=200) == balance(T=0x7fffffff, K=1) == -4
     assert L.mok_router_balance_scratch_bytes(0, 8, 1) == 0
     bwd = lambda *, g=p, T=512, E=8, K=2, S=1, top=0, w=0, dw=0, off=0: L.mok_router_balance_bwd(                              # noqa: E731
         L.pack_router_balance_bwd(g, p, p, 0, off, top, w, dw, p, 0, T, E, K, S, 0), None)
     assert bwd(g=0) == bwd(T=0) == bwd(S=3) == bwd(top=p) == bwd(top=p, w=p) == bwd(top=p, w=p, dw=p, K=33, E=64) == -1
     assert bwd(top=p, w=p, dw=p, K=9) == -1
-    assert bwd(E=2000) == -3
+    assert bwd(E=2000) == -3 and bwd(T=0x7fffffff) == bwd(S=1 << 30, off=p) == -4
     p = ctypes.c_void_p(4096)
     counts = lambda *, ids=p, T=512, E=8, K=2, S=1, off=z: L.mok_expert_counts(ids, 0, T, K, E, S, z, off, p, z)              # noqa: E731
     assert counts(ids=z) == counts(T=-1) == counts(E=0) == counts(S=2) == -1
