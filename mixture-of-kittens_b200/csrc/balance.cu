@@ -311,12 +311,15 @@ __device__ __forceinline__ float sigmoid_rest(float l) { return rcp_fast(1.0f + 
 // Of one row held by a group of kLanes lanes: ex = exponentials and inv the reciprocal of their sum (softmax = ex inv), for
 // sigmoid scores also sg = scaled sigmoids and inv_sg.  inv is 0 for a row without a logit above -inf, and lse then 0.
 struct RowStats { float inv, inv_sg, lse; };
-template <int kLanes, int V, bool kSigmoid>
-__device__ __forceinline__ RowStats row_stats(const float (&v)[V], float (&ex)[V], float (&sg)[V]) {
+template <int kLanes, int V>
+__device__ __forceinline__ float row_max(const float (&v)[V]) {              // NaN where there is nothing else
     float m = v[0];
 #pragma unroll
     for (int j = 1; j < V; ++j) m = fmaxf(m, v[j]);
-    m = group_max<kLanes>(m);
+    return group_max<kLanes>(m);
+}
+template <int kLanes, int V, bool kSigmoid>
+__device__ __forceinline__ RowStats row_stats(const float (&v)[V], float m, float (&ex)[V], float (&sg)[V]) {      // m: row_max, or -inf for NaN
     const float base = m > -INFINITY ? m : 0.0f;
     float sum = 0.0f;
 #pragma unroll
@@ -403,22 +406,32 @@ __device__ __forceinline__ float warp_min(float v) {
     return m;
 }
 
-// Values >= t into gathered[0..min(n, 32)), one slot each in no order that matters; returns how many there are.
+// Values >= t into gathered[0..min(n, 32)), one slot each in no order that matters; returns how many there are.  Written out so
+// that the store is predicated: as a branch a value it costs three instructions more.
 template <int V>
 __device__ __forceinline__ int gather_above(const float (&v)[V], float t, uint2* gathered) {
     const int lane = threadIdx.x & 31;
-    const unsigned below = (1u << lane) - 1u;
-    int n = 0;
+    const uint32_t below = (1u << lane) - 1u, base = smem_u32(gathered);
+    uint32_t n = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const bool in = v[j] >= t;
-        const unsigned at = __ballot_sync(kAll, in);
-        if (V <= 8 || at != 0) {
-            if (in) gathered[(n + __popc(at & below)) & 31] = make_uint2(Held<32, V>::expert(lane, j), __float_as_uint(v[j]));
-            n += __popc(at);
-        }
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b32 at, to;\n\t"
+            "setp.ge.f32 p, %1, %2;\n\t"
+            "vote.sync.ballot.b32 at, p, 0xffffffff;\n\t"
+            "and.b32 to, at, %3;\n\t"
+            "popc.b32 to, to;\n\t"
+            "add.u32 to, to, %0;\n\t"
+            "and.b32 to, to, 31;\n\t"
+            "mad.lo.u32 to, to, 8, %4;\n\t"
+            "@p st.shared.v2.b32 [to], {%5, %6};\n\t"
+            "popc.b32 at, at;\n\t"
+            "add.u32 %0, %0, at;\n\t}"
+            : "+r"(n)
+            : "f"(v[j]), "f"(t), "r"(below), "r"(base), "r"(Held<32, V>::expert(lane, j)), "r"(__float_as_uint(v[j]))
+            : "memory");
     }
-    return n;
+    return static_cast<int>(n);
 }
 
 // One row a warp.  Let the lanes form K sets of `set` neighbours, as large as they can be, and t be the least of the sets'
@@ -675,11 +688,13 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
                 load(t0, v);
             }
             const bool live = there && counted && (g.mask == nullptr || g.mask[t]);
+            float max_known;
             if constexpr (kSelect) {
-                const size_t o = static_cast<size_t>(t) * g.K;
+                const unsigned o = static_cast<unsigned>(t) * static_cast<unsigned>(g.K);        // a call has fewer than 2^31 routes
                 if constexpr (kLanes == 32) select_by_rank<V>(v, g.E, g.K, set, s_gathered[warp], chosen);
                 else select_in_rounds<kLanes, V>(v, g.E, g.K, chosen);
                 const float top = chosen[0].x;
+                max_known = top;
                 auto weight = [&](float x) {
                     return top == -INFINITY ? 0.0f : kSigmoid ? sigmoid_scaled(x, top) : exp2_fast((x - top) * kLog2e);
                 };
@@ -704,10 +719,12 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
                     }
                 }
                 __syncwarp();
+            } else {
+                max_known = row_max<kLanes, V>(v);
             }
             if (counted) {
                 float ex[V], sg[V];
-                const RowStats r = row_stats<kLanes, V, kSigmoid>(v, ex, sg);
+                const RowStats r = row_stats<kLanes, V, kSigmoid>(v, max_known, ex, sg);
                 if (live) {
 #pragma unroll
                     for (int j = 0; j < V; ++j) acc[j] = kSigmoid ? fmaf(sg[j], r.inv_sg, acc[j]) : fmaf(ex[j], r.inv, acc[j]);
@@ -891,7 +908,7 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) b
         }
         if (kLanes == 32 ? live : losses) {            // shorter groups of a warp stay in step
             float ex[V], sg[V];
-            const RowStats r = row_stats<kLanes, V, kSigmoid>(v, ex, sg);
+            const RowStats r = row_stats<kLanes, V, kSigmoid>(v, row_max<kLanes, V>(v), ex, sg);
             float dot = 0.0f;
 #pragma unroll
             for (int j = 0; j < V; ++j) dot = fmaf(kSigmoid ? sg[j] : ex[j], a[j], dot);
