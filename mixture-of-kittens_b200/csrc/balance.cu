@@ -36,6 +36,7 @@ constexpr int row_blocks_per_sm(int E) { return E <= 512 ? 2 : 1; }
 constexpr int kCluster = 8;                    // blocks of a forward pass in one launch
 constexpr int kMinCols = 8;                    // fewest experts of a join tile
 constexpr unsigned kAll = 0xffffffffu;
+enum : int { kNone = 0, kFew = 1, kMany = 2 };      // routes that a launch chooses: finished ones, up to 16, more
 
 struct SlotHead { float z; int rows, routes, pad; };
 
@@ -434,6 +435,15 @@ __device__ __forceinline__ int gather_above(const float (&v)[V], float t, uint2*
     return static_cast<int>(n);
 }
 
+// The largest sets of lanes of which there are K (one of which half the lanes have values counts); 0: there are none.
+template <int V>
+__device__ __forceinline__ int set_of(int E, int K) {
+    const int lanes = min(32, (E + Held<32, V>::kUnit - 1) / Held<32, V>::kUnit);
+    int set = 32;
+    while (set > 0 && (lanes + set / 2) / set < K) set >>= 1;
+    return set;
+}
+
 // One row a warp.  Let the lanes form K sets of `set` neighbours, as large as they can be, and t be the least of the sets'
 // maxima: at least K values are >= t, and few more.  They are gathered, one a lane, and every lane counts those that come
 // before its own.  Where more than 32 are >= t (with K = 8 of 256 in 8 rows of 100), t is the K-th largest of the lanes' maxima
@@ -480,6 +490,25 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
     }
     if (lane < n && before < K) chosen[before] = make_float2(__uint_as_float(own.y), __int_as_float(static_cast<int>(own.x)));
     __syncwarp();
+}
+
+// More than 16 of a row would rarely leave 32 or fewer values >= t: 16 are chosen at a time and taken out of v (131072 x 256, 32 of
+// them: 444 us in rounds, 238 so; in kernels of their own, because the code beside it costs the choice of fewer 14 % and more).
+template <int V>
+__device__ __forceinline__ void select_many(float (&v)[V], int E, int K, uint2* gathered, float2* chosen) {
+    const int lane = threadIdx.x & 31;
+    int above = 0;                                                 // values above -inf; with fewer than K the choice goes beyond them
+#pragma unroll
+    for (int j = 0; j < V; ++j) above += __popc(__ballot_sync(kAll, v[j] > -INFINITY));
+    if (above < K) { select_in_rounds<32, V>(v, E, K, chosen); return; }
+    for (int from = 0; from < K; from += 16) {
+        const int some = min(K - from, 16);
+        select_by_rank<V>(v, E, some, set_of<V>(E, some), gathered, chosen + from);
+        const float2 last = chosen[from + some - 1];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (v[j] > last.x || (v[j] == last.x && Held<32, V>::expert(lane, j) <= __float_as_int(last.y))) v[j] = -INFINITY;
+    }
 }
 
 __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(kAll, v); }
@@ -615,15 +644,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) balance_join_kernel(const Bal
 }
 
 // Bound by instructions and, without the choice, by the latency of its loads.  Reads T E logits once, writes K routes a row and (p,
-// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 78 (21), finished routes
-// 36; 65536 x 500 bf16, K = 6, 61 sequences: 69 (10) and 32; 16384 x 128: 16 (1.3) and 10.  A row of 256 takes 500 instructions
-// with the choice, 180 without; in rounds of one maximum each the choice alone took 540.  Loading the next row ahead: 53 -> 44
+// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 75 (21), finished routes
+// 36; 65536 x 500 bf16, K = 6, 61 sequences: 69 (10) and 32; 16384 x 128: 16 (1.3) and 10.  A row of 256 takes 470 instructions
+// with the choice, 130 without; in rounds of one maximum each the choice alone took 540.  Loading the next row ahead: 53 -> 44
 // without the choice at 256 experts; above, the registers it takes cost more (36 -> 46 at 500).  Finished routes are counted for a
 // run's rows at once; with their row, each row waited for its ids (44 -> 36).  Rows staged in shared memory two to four ahead by
 // asynchronous copies were slower throughout (44 -> 55, backward 54 -> 73 to 77).
-template <typename T, int kLanes, int V, bool kSigmoid, bool kSelect>
+template <typename T, int kLanes, int V, bool kSigmoid, int kChoose>
 __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) balance_rows_kernel(const BalanceParams g) {
     using Row = SharedRow<kLanes, V>;
+    constexpr bool kSelect = kChoose != kNone;
     constexpr bool kAhead = V <= 8;            // the next row is loaded while this one is worked on
     constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // chosen experts a lane, at most (K <= 32 and <= E)
@@ -636,10 +666,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
     float2* const chosen = reinterpret_cast<float2*>(hist + ((g.E + 1) & ~1)) + static_cast<size_t>(group) * g.K;
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0 && !g.one_launch) *g.ticket = 0;
-    // select_by_rank: the largest sets of lanes of which there are K (one of which half the lanes have values counts)
-    const int lanes = min(32, (g.E + Held<kLanes, V>::kUnit - 1) / Held<kLanes, V>::kUnit);
-    int set = 32;
-    while (set > 0 && (lanes + set / 2) / set < g.K) set >>= 1;
+    const int set = kLanes == 32 && kChoose == kFew ? set_of<V>(g.E, g.K) : 0;
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
@@ -691,8 +718,14 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
             float max_known;
             if constexpr (kSelect) {
                 const unsigned o = static_cast<unsigned>(t) * static_cast<unsigned>(g.K);        // a call has fewer than 2^31 routes
-                if constexpr (kLanes == 32) select_by_rank<V>(v, g.E, g.K, set, s_gathered[warp], chosen);
-                else select_in_rounds<kLanes, V>(v, g.E, g.K, chosen);
+                if constexpr (kLanes != 32) {
+                    select_in_rounds<kLanes, V>(v, g.E, g.K, chosen);
+                } else if constexpr (kChoose == kFew) {
+                    select_by_rank<V>(v, g.E, g.K, set, s_gathered[warp], chosen);
+                } else {
+                    select_many<V>(v, g.E, g.K, s_gathered[warp], chosen);
+                    load(t0, v);                                   // as it was
+                }
                 const float top = chosen[0].x;
                 max_known = top;
                 auto weight = [&](float x) {
@@ -1039,11 +1072,11 @@ __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const Coun
     }
 }
 
-template <typename T, int kLanes, int V, bool kSigmoid, bool kSelect>
+template <typename T, int kLanes, int V, bool kSigmoid, int kChoose>
 int launch_rows(const BalanceParams& p, cudaStream_t s) {
-    const size_t chosen = kSelect ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
+    const size_t chosen = kChoose != kNone ? static_cast<size_t>(2) * (kRowThreads / kLanes) * p.K : 0;
     const size_t smem = (static_cast<size_t>(kSumRows) * SharedRow<kLanes, V>::kFloats + ((p.E + 1) & ~1) + chosen) * 4;
-    if (!p.one_launch) return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid, kSelect>, p.blocks, kRowThreads, smem, s, false, true, p);
+    if (!p.one_launch) return launch_kernel(balance_rows_kernel<T, kLanes, V, kSigmoid, kChoose>, p.blocks, kRowThreads, smem, s, false, true, p);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kCluster);
     cfg.blockDim = dim3(kRowThreads);
@@ -1056,15 +1089,20 @@ int launch_rows(const BalanceParams& p, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    auto* kern = balance_rows_kernel<T, kLanes, V, kSigmoid, kSelect>;
+    auto* kern = balance_rows_kernel<T, kLanes, V, kSigmoid, kChoose>;
     MOK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
     return MOK_OK;
 }
 
+template <typename T, int kLanes, int V, bool kSigmoid>
+int launch_choice(const BalanceParams& p, cudaStream_t s) {
+    if (p.top_in != nullptr) return launch_rows<T, kLanes, V, kSigmoid, kNone>(p, s);
+    if constexpr (kLanes == 32) if (p.K > 16) return launch_rows<T, kLanes, V, kSigmoid, kMany>(p, s);
+    return launch_rows<T, kLanes, V, kSigmoid, kFew>(p, s);
+}
 template <typename T, int kLanes, int V>
 int launch_rows_as(const BalanceParams& p, cudaStream_t s) {
-    if (p.top_in == nullptr) return p.sigmoid ? launch_rows<T, kLanes, V, true, true>(p, s) : launch_rows<T, kLanes, V, false, true>(p, s);
-    return p.sigmoid ? launch_rows<T, kLanes, V, true, false>(p, s) : launch_rows<T, kLanes, V, false, false>(p, s);
+    return p.sigmoid ? launch_choice<T, kLanes, V, true>(p, s) : launch_choice<T, kLanes, V, false>(p, s);
 }
 
 template <typename T, int kLanes, int V, bool kSigmoid>

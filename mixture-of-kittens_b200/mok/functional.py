@@ -419,7 +419,8 @@ def balance_loss(logits: torch.Tensor, top_experts: torch.Tensor, *, token_mask:
                  group: dist.ProcessGroup | None = None) -> MoKBalance:
     """Balance loss, z-loss and per-expert counts of finished routes (int64 [T, K]) and the logits behind them (f32 or bf16
     [T, E]); see `ops.router_balance`.  With `group` the loss uses the counts of all its ranks (one all-reduce of [1, E]
-    int32; averaged over the ranks the loss is then that of the global batch); `counts` stays local."""
+    int32; averaged over ranks with as many tokens that count each, it is the loss of the global batch); `counts` stays
+    local."""
     sigmoid = _sigmoid_score(score)
     load = None
     if group is not None:

@@ -103,7 +103,8 @@ def check(dev, logits, K, where, sigmoid, *, experts=None, load=None, with_weigh
 
 
 SHAPES = [(1, 1, 1), (1, 7, 3), (3, 8, 2), (17, 4, 4), (255, 16, 2), (513, 24, 5), (300, 33, 32), (1000, 64, 6), (777, 100, 7),
-          (2049, 128, 8), (640, 255, 8), (511, 256, 9), (300, 500, 6), (130, 512, 31), (200, 1000, 8), (97, 1024, 32)]
+          (2049, 128, 8), (640, 255, 8), (511, 256, 9), (300, 500, 6), (130, 512, 31), (200, 1000, 8), (97, 1024, 32), (333, 256, 32),
+          (200, 70, 20), (150, 128, 17), (90, 300, 16)]
 
 
 @pytest.mark.parametrize("sigmoid", [False, True])
@@ -205,6 +206,19 @@ def test_rows_of_the_lowest_value(cuda_device, E, dtype, sigmoid):
         a = O.expert_counts(chosen, E) * E / counts.sum().item() / T
         scale = 2 * torch.from_numpy(a).max() + 2.0 ** -20       # weights of a row add up to 1 within WEIGHT
         assert float((got.cpu().double() - grad).abs().max()) <= (GRAD + (2.0 ** -8 if dtype == torch.bfloat16 else 0)) * float(scale) + WEIGHT
+
+
+@pytest.mark.parametrize("E", [70, 128, 256, 600])
+def test_many_routes_among_equal_and_missing_logits(cuda_device, E):
+    """More than 16 routes with ties across the 16th, with just enough, and with too few logits above -inf."""
+    K, T = 30, 24
+    logits = make(cuda_device, T, E, K, seed=E)[0]
+    logits[0:4] = torch.round(logits[0:4])
+    logits[4] = 0.0
+    for row, left in ((5, 30), (6, 29), (7, 17), (8, 16), (9, 15), (10, 1), (11, 0)):
+        logits[row, torch.randperm(E, generator=torch.Generator().manual_seed(row))[left:]] = -np.inf
+    for sigmoid in (False, True):
+        check(cuda_device, logits, K, {}, sigmoid)
 
 
 def test_far_below_zero_sigmoids_do_not_vanish(cuda_device):
