@@ -534,3 +534,37 @@ def test_compiled_and_threaded_calls(cuda_device):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not failed, failed
+
+
+def test_captured_behind_copies_and_other_streams(cuda_device):
+    """In a graph, calls whose neighbours are a memset, a copy, and work of another stream that they wait for."""
+    from mok import ops
+    source = make(cuda_device, 3000, 96, 5, seed=31)[0].to(cuda_device)
+    x, seed = torch.zeros_like(source), torch.tensor([3], device=cuda_device)
+    want = ops.router_topk_balance(source, 5)
+    want_grad = ops.router_balance_bwd(want[2], source, want[4], None, None, want[0], want[1], want[1])
+    want_drop = ops.dropout_add(source, source, seed, 0.25)
+    side = torch.cuda.Stream(cuda_device)
+    pool = torch.cuda.Stream(cuda_device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=pool):
+        x.zero_()
+        x.copy_(source)
+        out = ops.router_topk_balance(x, 5)
+        side.wait_stream(pool)
+        with torch.cuda.stream(side):
+            drop = ops.dropout_add(x, x, seed, 0.25)
+            counts = ops.expert_counts(out[0], 96)
+        pool.wait_stream(side)
+        grad = ops.router_balance_bwd(out[2], x, out[4], None, None, out[0], out[1], out[1])
+        drop2 = drop.clone()
+        x.zero_()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out)) and torch.equal(grad, want_grad)
+        assert torch.equal(drop, want_drop) and torch.equal(drop2, want_drop) and torch.equal(counts[0], want[3][0])
+        assert int(x.count_nonzero()) == 0
+        for t in (*out, grad, drop, drop2, counts):
+            t.zero_()
