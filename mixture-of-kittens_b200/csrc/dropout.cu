@@ -20,10 +20,13 @@ constexpr int kDropThreads = 64;
 
 // Groups of eight elements that a thread has in flight, and blocks that an SM has to be able to hold (which bounds the
 // registers).  The kernel moves bytes and, in bf16, draws numbers nearly as long as it moves them, so it needs many loads in
-// flight and few warps to issue them from; with more resident warps DRAM gets slower again.  One B200, 16384 x 7168 bf16, us
-// without dependent launches, which take 2 us more off (floor: bytes at the measured copy rate of 6456 GB/s): with a residual (109) 6 groups, 10 blocks 106; 5, 10: 108; 6, 12: 112;
-// 256 threads, 4 groups, 3 blocks: 112; 256 threads, 2 groups: 118 to 130.  Without one (73) 7, 12: 75.5; 8, 12: 77; 6, 12: 80;
-// 5, 10: 89; 256 threads: 83 to 105.  f32, 10000 x 2042 (38.0 and 25.3): 2, 8: 38.7 and 27.4; 3, 12: 39.7 and 27.4; 4, 10: 41.7 and 27.4.
+// flight and few warps to issue them from; with more resident warps DRAM gets slower again.  One B200, us, groups and blocks
+// (floor: bytes at the measured copy rate of 6456 GB/s), without dependent launches, which take 2 us more off:
+//   16384 x 7168 bf16 with a residual (109):  6, 10: 106;  5, 10: 108;  6, 12: 112;  256 threads: 112 to 130
+//   the same without one (73):                7, 12: 75.5;  8, 12: 77;  6, 12: 80;  5, 10: 89;  256 threads: 83 to 105
+//   10000 x 2042 f32 (38.0 and 25.3):         2, 8: 38.7 and 27.4;  3, 12: 39.7 and 27.4;  4, 10: 41.7 and 27.4
+// Inputs are read past the cache (they are not needed again), the result is not: whoever reads it next finds part of it there.
+// With an elementwise kernel behind it, 16384 x 2048 bf16: 57.6 us with both past the cache, 55 so, 56 with neither.
 template <typename T, bool kResidual> struct Shape {
     static constexpr int kUnroll = sizeof(T) == 4 ? 2 : kResidual ? 6 : 7;
     static constexpr int kBlocks = sizeof(T) == 4 ? 8 : kResidual ? 10 : 12;
@@ -68,7 +71,7 @@ template <> struct Eight<__nv_bfloat16> {
         for (int i = 0; i < 4; ++i) { const float2 t = unpack_bf16(w[i]); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
     }
     static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[8]) {
-        __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])));
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
     }
 };
 template <> struct Eight<float> {
@@ -81,8 +84,8 @@ template <> struct Eight<float> {
         f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
     }
     static __device__ __forceinline__ void store(float* p, const float (&f)[8]) {
-        __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
-        __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(f[4], f[5], f[6], f[7]));
+        *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
     }
 };
 
