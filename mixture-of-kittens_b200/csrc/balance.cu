@@ -445,9 +445,11 @@ __device__ __forceinline__ int set_of(int E, int K) {
 }
 
 // One row a warp.  Let the lanes form K sets of `set` neighbours, as large as they can be, and t be the least of the sets'
-// maxima: at least K values are >= t, and few more.  They are gathered, one a lane, and every lane counts those that come
-// before its own.  Where more than 32 are >= t (with K = 8 of 256 in 8 rows of 100), t is the K-th largest of the lanes' maxima
-// instead, and where that does not do either (many equal values, few above -inf, no such sets: set = 0) the row goes in rounds.
+// maxima: at least K values are >= t, and few more.  They are gathered, one a lane, and every lane counts those that come before
+// its own.  With t the second, third or fourth least for more routes there are fewer to gather and still nearly always K (8 of 256,
+// second least: 13 on average, fewer than 8 in 2 rows of 100; least: 21, more than 32 in 9 of 100).  In the rows where that fails t
+// is the K-th largest of the lanes' maxima, and where that does not do either (many equal values, few above -inf, no such sets:
+// set = 0) the row goes in rounds.
 template <int V>
 __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K, int set, uint2* gathered, float2* chosen) {
     const int lane = threadIdx.x & 31;
@@ -457,10 +459,15 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
     b = b > -INFINITY ? b : -INFINITY;                             // all NaN
     float t = b;
     for (int off = 1; off < set; off <<= 1) t = fmaxf(t, __shfl_xor_sync(kAll, t, off));
-    t = warp_min(lane < K * set ? t : INFINITY);
+    float least = lane < K * set ? t : INFINITY;
+    t = warp_min(least);
+    for (int i = K < 5 ? 0 : K < 11 ? 1 : K < 15 ? 2 : 3; i > 0; --i) {
+        least = least == t ? INFINITY : least;
+        t = warp_min(least);
+    }
     int n = 33;
     if (set > 0 && t > -INFINITY) n = gather_above(v, t, gathered);
-    if (n > 32) {
+    if (n > 32 || n < K) {
         int found = 0;
         do {
             t = group_max<32>(b);
@@ -469,7 +476,7 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
             b = equal ? -INFINITY : b;
         } while (found < K && t > -INFINITY);
         __syncwarp();
-        if (t > -INFINITY) n = gather_above(v, t, gathered);
+        n = t > -INFINITY ? gather_above(v, t, gathered) : 33;
         if (n > 32) { select_in_rounds<32, V>(v, E, K, chosen); return; }
     }
     __syncwarp();
@@ -493,7 +500,7 @@ __device__ __forceinline__ void select_by_rank(const float (&v)[V], int E, int K
 }
 
 // More than 16 of a row would rarely leave 32 or fewer values >= t: 16 are chosen at a time and taken out of v (131072 x 256, 32 of
-// them: 444 us in rounds, 238 so; in kernels of their own, because the code beside it costs the choice of fewer 14 % and more).
+// them: 444 us in rounds, 179 so; in kernels of their own, because the code beside it costs the choice of fewer 14 % and more).
 template <int V>
 __device__ __forceinline__ void select_many(float (&v)[V], int E, int K, uint2* gathered, float2* chosen) {
     const int lane = threadIdx.x & 31;
@@ -644,7 +651,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) balance_join_kernel(const Bal
 }
 
 // Bound by instructions and, without the choice, by the latency of its loads.  Reads T E logits once, writes K routes a row and (p,
-// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 75 (21), finished routes
+// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 74 (21), finished routes
 // 36; 65536 x 500 bf16, K = 6, 61 sequences: 69 (10) and 32; 16384 x 128: 16 (1.3) and 10.  A row of 256 takes 470 instructions
 // with the choice, 130 without; in rounds of one maximum each the choice alone took 540.  Loading the next row ahead: 53 -> 44
 // without the choice at 256 experts; above, the registers it takes cost more (36 -> 46 at 500).  Finished routes are counted for a
