@@ -105,13 +105,6 @@ __device__ __forceinline__ float group_max(float v) {       // a NaN loses again
     for (int off = kLanes / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, off));
     return v;
 }
-template <int kLanes>
-__device__ __forceinline__ int group_min(int v) {
-    if constexpr (kLanes == 32) return __reduce_min_sync(kAll, v);
-#pragma unroll
-    for (int off = kLanes / 2; off > 0; off >>= 1) v = min(v, __shfl_xor_sync(kAll, v, off));
-    return v;
-}
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -28,41 +28,39 @@ __device__ __forceinline__ void two_largest(const float (&v)[V], unsigned taken,
 // The K largest values of a row, descending, the lower expert first among equals, into chosen[0..K) (shared memory of the
 // group) as (value, expert).
 //
-// In rounds: every lane keeps the two largest values it has left; a round is one maximum over the group, the winner moves its
-// second up, and a lane that has used up both looks through its values again (with K = 8 of 256 over 32 lanes in half of
-// the rows; one kept value would mean a search in every round).
-template <int kLanes, int V>
+// In rounds, one row a warp: every lane keeps the two largest values it has left; a round is one maximum over the warp, the winner
+// moves its second up, and a lane that has used up both looks through its values again (with K = 8 of 256 in half of the rows; one
+// kept value would mean a search in every round).
+template <int V>
 __device__ __forceinline__ void select_in_rounds(const float (&v)[V], int E, int K, float2* chosen) {
-    const int lane = threadIdx.x & 31, l = lane % kLanes;
-    const unsigned group = kLanes == 32 ? kAll : ((1u << kLanes) - 1u) << (lane - l);
+    using At = Held<32, V>;
+    const int lane = threadIdx.x & 31;
     const unsigned below = (1u << lane) - 1u;
-    using At = Held<kLanes, V>;
-    const int mine = At::count(l, E);
+    const int mine = At::count(lane, E);
     unsigned taken = 0;
     float b1, b2;
     int j1, j2;
     two_largest(v, 0u, b1, j1, b2, j2);
     for (int k = 0; k < K; ++k) {
-        const float best = group_max<kLanes>(b1);
+        const float best = group_max<32>(b1);
         const bool equal = j1 < V && b1 == best;
-        const unsigned at = __ballot_sync(kAll, equal) & group;
+        const unsigned at = __ballot_sync(kAll, equal);
         bool win = equal && (at & below) == 0;
-        if (V > At::kUnit && __any_sync(kAll, (at & (at - 1)) != 0)) {          // equals in several lanes, whose experts interleave
-            const int e = equal ? At::expert(l, j1) : 0x7fffffff;
-            win = e == group_min<kLanes>(e) && equal;
+        if (V > At::kUnit && (at & (at - 1)) != 0) {               // equals in several lanes, whose experts interleave
+            const int e = equal ? At::expert(lane, j1) : 0x7fffffff;
+            win = e == __reduce_min_sync(kAll, e) && equal;
         }
-        if (win) chosen[k] = make_float2(best, __int_as_float(At::expert(l, j1)));
+        if (win) chosen[k] = make_float2(best, __int_as_float(At::expert(lane, j1)));
         taken |= win ? 1u << (j1 & 31) : 0u;
         const bool dry = win && j2 == V;
         b1 = win ? b2 : b1;
         j1 = win ? j2 : j1;
         b2 = win ? -INFINITY : b2;
         j2 = win ? V : j2;
-        if (__any_sync(kAll, at == 0)) {                           // nothing above -inf left: the lowest experts not taken yet
+        if (at == 0) {                                             // nothing above -inf left: the lowest expert not taken yet
             const unsigned left = ~taken & (V == 32 && mine == 32 ? kAll : (1u << mine) - 1u);
-            const int e = left ? At::expert(l, __ffs(left) - 1) : 0x7fffffff;
-            const int lowest = group_min<kLanes>(e);
-            if (at == 0 && e == lowest && left) { chosen[k] = make_float2(-INFINITY, __int_as_float(e)); taken |= left & (0u - left); }
+            const int e = left ? At::expert(lane, __ffs(left) - 1) : 0x7fffffff;
+            if (e == __reduce_min_sync(kAll, e) && left) { chosen[k] = make_float2(-INFINITY, __int_as_float(e)); taken |= left & (0u - left); }
         }
         if (__any_sync(kAll, dry)) { if (dry) two_largest(v, taken, b1, j1, b2, j2); }
     }
@@ -111,7 +109,7 @@ __device__ __forceinline__ void select_sorted(const float (&v)[4], int E, int K,
 template <int kLanes, int V>
 __device__ __forceinline__ void rounds(const float (&v)[V], int E, int K, float2* chosen) {
     if constexpr (V == 4) select_sorted<kLanes>(v, E, K, chosen);
-    else select_in_rounds<kLanes, V>(v, E, K, chosen);
+    else select_in_rounds<V>(v, E, K, chosen);                     // rows of more than four values a lane have a warp each
 }
 
 __device__ __forceinline__ float warp_min(float v) {
