@@ -172,7 +172,8 @@ int mok_router_topk_bwd(const int32_t* top_experts_i32, const float* router_weig
  * num_tokens * topk stays below 2^31 - 2^16.
  * load: int32 [num_sequences, E] that stands for the counts in f, a sequence's sum below 2^31 (NULL: the counts).  Outputs: losses f32 [2], counts int32
  * [num_sequences, E], coef f32 [num_sequences * E + 2] for mok_router_balance_bwd.  scratch: 16-byte aligned,
- * mok_router_balance_scratch_bytes bytes (0: none is needed, NULL will do), of this call alone until it has run.
+ * mok_router_balance_scratch_bytes bytes (0: none is needed, NULL will do; chooses: top_experts_in is NULL), of this call
+ * alone until it has run.
  * mok_router_balance_bwd writes all of d_logits (type of logits) from d_losses f32 [2] and, where the three are not NULL,
  * from the gradient of the router weights (topk <= 32 and <= num_experts).
  * No reference counterpart (the reference takes finished routes and returns no losses). */
@@ -203,7 +204,7 @@ typedef struct mok_router_balance_bwd_args {
     void* d_logits;
     int logits_bf16, num_tokens, num_experts, topk, num_sequences, sigmoid;
 } mok_router_balance_bwd_args;
-size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences);
+size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences, int chooses);
 int mok_router_balance(const mok_router_balance_args* args, void* stream);
 int mok_router_balance_bwd(const mok_router_balance_bwd_args* args, void* stream);
 

@@ -39,17 +39,22 @@ struct Scratch {
 // rows that a block works on at once
 int rows_at_once(int E) { return kWarps * (E <= 16 ? 8 : E <= 32 ? 4 : E <= 64 ? 2 : 1); }
 // One launch of one cluster that joins its blocks' sums through shared memory and needs no scratch, or one launch of many
-// blocks and one that joins their slots.  Up to two rows a group of lanes the cluster saves the caller a launch and an
-// allocation, 4 us of its time; the device takes 6.5 us for one row a group and 7.1 to 9.8 for two, against 7 to 9.5 with two launches.
-bool in_one_launch(int T, int E, int S) { return S == 1 && T <= 2 * kCluster * rows_at_once(E); }
-int rows_per_block(int T, int E, int S) {
-    const int most = in_one_launch(T, E, S) ? kCluster : 148 * row_blocks_per_sm(E), at_once = rows_at_once(E);
+// blocks and one that joins their slots.  The limit is in rows a group of lanes, where the device's times meet; the cluster also saves
+// the caller a launch and an allocation, 4 us of its time.  One B200, us, cluster and two launches, choosing K = 2 to 8 / with
+// finished routes: 8 experts 1 row 5.4 and 6.7 / 5.0 and 7.4, 3 rows 7.3 and 6.7 / 5.9 and 7.5, 6 rows 10.1 and 7.3 / 7.0 and 7.0; 128 experts
+// 3 rows 8.3 and 8.5 / 5.7 and 7.3, 6 rows 11.8 and 8.6 / 6.9 and 7.4; 1000 experts 1 row 10.4 and 11.7 / 7.8 and 8.9, 2 rows 13.9 and 11.8 / 8.7 and 9.1.
+bool in_one_launch(int T, int E, int S, bool choose) {
+    const int rows = E > 512 ? (choose ? 1 : 2) : (choose ? 3 : 6);
+    return S == 1 && T <= rows * kCluster * rows_at_once(E);
+}
+int rows_per_block(int T, int E, int S, bool choose) {
+    const int most = in_one_launch(T, E, S, choose) ? kCluster : 148 * row_blocks_per_sm(E), at_once = rows_at_once(E);
     const int rows = (T + most - 1) / most;
     return (rows + at_once - 1) / at_once * at_once;
 }
-int row_blocks(int T, int E, int S) {
-    if (in_one_launch(T, E, S)) return kCluster;
-    const int rows = rows_per_block(T, E, S);
+int row_blocks(int T, int E, int S, bool choose) {
+    if (in_one_launch(T, E, S, choose)) return kCluster;
+    const int rows = rows_per_block(T, E, S, choose);
     return (T + rows - 1) / rows;
 }
 
@@ -250,10 +255,10 @@ bool too_many_routes(int T, int K) { return T > 0x7fff0000 || static_cast<long l
 using namespace mok;
 using namespace mok::balance;
 
-extern "C" size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences) {
+extern "C" size_t mok_router_balance_scratch_bytes(int num_tokens, int num_experts, int num_sequences, int chooses) {
     if (bad_sizes(num_tokens, num_experts, 1, num_sequences)) return 0;
-    if (in_one_launch(num_tokens, num_experts, num_sequences)) return 0;
-    return Scratch(nullptr, row_blocks(num_tokens, num_experts, num_sequences) + num_sequences, num_experts, num_sequences).bytes;
+    if (in_one_launch(num_tokens, num_experts, num_sequences, chooses != 0)) return 0;
+    return Scratch(nullptr, row_blocks(num_tokens, num_experts, num_sequences, chooses != 0) + num_sequences, num_experts, num_sequences).bytes;
 }
 
 extern "C" int mok_router_balance(const mok_router_balance_args* args, void* stream) {
@@ -267,8 +272,9 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
     if (E > 1024) return MOK_ERR_UNSUPPORTED;
     if (too_many_routes(T, K) || static_cast<long long>(S) * E > 0x7fffffff) return MOK_ERR_TOO_LARGE;
     BalanceParams p{};
-    p.blocks = row_blocks(T, E, S);
-    p.one_launch = in_one_launch(T, E, S);
+    const bool choose = a.top_experts_in == nullptr;
+    p.blocks = row_blocks(T, E, S, choose);
+    p.one_launch = in_one_launch(T, E, S, choose);
     const Scratch at(a.scratch, p.blocks + S, E, S);
     if (!p.one_launch && (!a.scratch || a.scratch_bytes < at.bytes || reinterpret_cast<uintptr_t>(a.scratch) % 16)) return MOK_ERR_INVALID;
     p.logits = a.logits;
@@ -282,7 +288,7 @@ extern "C" int mok_router_balance(const mok_router_balance_args* args, void* str
     p.counts = a.counts;
     p.coef = a.coef;
     p.T = T; p.E = E; p.K = K; p.S = S;
-    p.rows_per_block = rows_per_block(T, E, S);
+    p.rows_per_block = rows_per_block(T, E, S, choose);
     p.sigmoid = a.sigmoid;
     p.chunk = chunk_of(a.logits, E, a.logits_bf16 ? 2 : 4);
     p.head = at.head; p.slot_p = at.p; p.slot_routes = at.routes; p.part = at.part; p.seq_z = at.seq_z; p.seq_rows = at.seq_rows;

@@ -136,7 +136,7 @@ mok_fwd_epilogue = _sig("mok_fwd_epilogue", C.c_int, [vp, vp, vp, vp, C.c_int, C
 mok_bwd_epilogue = _sig("mok_bwd_epilogue", C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, vp])
 mok_router_topk = _sig("mok_router_topk", C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, vp, vp, u64p, C.c_int, C.c_int, vp])
 mok_router_topk_bwd = _sig("mok_router_topk_bwd", C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp])
-mok_router_balance_scratch_bytes = _sig("mok_router_balance_scratch_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int])
+mok_router_balance_scratch_bytes = _sig("mok_router_balance_scratch_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int])
 # the argument structs of these two as bytes: packing them costs a third of passing that many arguments
 pack_router_balance = struct.Struct("11PN6i").pack
 pack_router_balance_bwd = struct.Struct("9P6i").pack

@@ -991,7 +991,7 @@ def _run_balance(logits: Tensor, T: int, E: int, K: int, top_in: int, experts: i
     losses = torch.empty(2, dtype=_F32, device=dev)
     counts = torch.empty(S, E, dtype=_I32, device=dev)
     coef = torch.empty(S * E + 2, dtype=_F32, device=dev)
-    nbytes = _balance_scratch_bytes(T, E, S)
+    nbytes = _balance_scratch_bytes(T, E, S, top_in == 0)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.launch(dev, what, _lib.mok_router_balance, _lib.pack_router_balance(
         logits.data_ptr(), top_in, experts, weights, 0 if token_mask is None else token_mask.data_ptr(),

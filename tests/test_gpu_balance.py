@@ -150,9 +150,11 @@ def test_one_sequence_inside_a_small_batch(cuda_device, E, K, offsets):
 @pytest.mark.parametrize("E", [8, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 512, 513, 1024])
 def test_batches_around_the_sizes_where_the_kernels_change(cuda_device, E):
     at_once = 16 * (8 if E <= 16 else 4 if E <= 32 else 2 if E <= 64 else 1)
-    for T in (8 * at_once - 1, 16 * at_once, 16 * at_once + 1):
-        logits, where = make(cuda_device, T, E, 3, seed=T, mask=True)
-        check(cuda_device, logits, 3, where, T % 2 == 0)
+    for passes in (1, 2, 3, 6):
+        for T in (8 * passes * at_once, 8 * passes * at_once + 1):
+            logits, where = make(cuda_device, T, E, 3, seed=T, mask=True)
+            check(cuda_device, logits, 3, where, T % 2 == 0)
+            check(cuda_device, logits, 3, where, T % 2 == 0, experts=O.select(logits.numpy(), 3))
 
 
 def test_many_rows_and_few_experts(cuda_device):

@@ -120,9 +120,11 @@ def test_c_entries_refuse_bad_arguments():
     assert balance(top=0, out=p, w=p, K=9) == balance(top=0, out=p, w=p, E=64, K=33) == -1
     many = dict(T=100000, E=64)
     assert balance(n=64, **many) == balance(scratch=4104, **many) == balance(scratch=0, **many) == -1
-    assert L.mok_router_balance_scratch_bytes(512, 8, 1) == 0 < L.mok_router_balance_scratch_bytes(100000, 64, 1)
+    for chooses in (0, 1):
+        assert L.mok_router_balance_scratch_bytes(512, 8, 1, chooses) == 0 < L.mok_router_balance_scratch_bytes(100000, 64, 1, chooses)
+    assert L.mok_router_balance_scratch_bytes(2816, 24, 1, 0) == 0 < L.mok_router_balance_scratch_bytes(2816, 24, 1, 1)
     assert balance(E=1025) == -3 and balance(T=1 << 24, K=200) == balance(T=0x7fffffff, K=1) == -4
-    assert L.mok_router_balance_scratch_bytes(0, 8, 1) == 0
+    assert L.mok_router_balance_scratch_bytes(0, 8, 1, 0) == 0
     bwd = lambda *, g=p, T=512, E=8, K=2, S=1, top=0, w=0, dw=0, off=0: L.mok_router_balance_bwd(                              # noqa: E731
         L.pack_router_balance_bwd(g, p, p, 0, off, top, w, dw, p, 0, T, E, K, S, 0), None)
     assert bwd(g=0) == bwd(T=0) == bwd(S=3) == bwd(top=p) == bwd(top=p, w=p) == bwd(top=p, w=p, dw=p, K=33, E=64) == -1
