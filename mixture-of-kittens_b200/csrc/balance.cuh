@@ -38,7 +38,7 @@ constexpr int kSumRows = kWarps / 2;           // rows of E sums in shared memor
 constexpr int row_blocks_per_sm(int E) { return E <= 512 ? 2 : 1; }
 constexpr int kCluster = 8;                    // blocks of a forward pass in one launch
 constexpr unsigned kAll = 0xffffffffu;
-enum : int { kNone = 0, kFew = 1, kMany = 2 };      // routes that a launch chooses: finished ones, up to 16, more
+enum : int { kNone = 0, kRounds = 1, kRank = 2, kMany = 3 };      // how a launch chooses its routes (kNone: they are finished)
 
 struct SlotHead { float z; int rows, routes, pad; };
 

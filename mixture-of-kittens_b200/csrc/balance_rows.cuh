@@ -231,7 +231,7 @@ __device__ __forceinline__ void select_many(float (&v)[V], int E, int K, uint2* 
 
 // Bound by instructions and, without the choice, by the latency of its loads.  Reads T E logits once, writes K routes a row and (p,
 // routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 74 (21), finished routes
-// 36; 65536 x 500 bf16, K = 6, 61 sequences: 69 (10) and 32; 16384 x 128: 16 (1.3) and 10.  A row of 256 takes 470 instructions
+// 36; 65536 x 500 bf16, K = 6, 61 sequences: 69 (10) and 32; 16384 x 128: 15 (1.3) and 10.  A row of 256 takes 470 instructions
 // with the choice, 130 without; in rounds of one maximum each the choice alone took 540.  Loading the next row ahead: 53 -> 44
 // without the choice at 256 experts; above, the registers it takes cost more (36 -> 46 at 500).  Finished routes are counted for a
 // run's rows at once; with their row, each row waited for its ids (44 -> 36).  Rows staged in shared memory two to four ahead by
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
     constexpr int kGroups = kRowThreads / kLanes;              // rows that a block works on at once
     constexpr int kPer = (kLanes * V < 32 ? kLanes * V : 32) / kLanes;          // chosen experts a lane, at most (K <= 32 and <= E)
     extern __shared__ __align__(16) float smem[];               // sums of p [kSumRows], routes [E], then the chosen (value, expert) [kGroups][K]
-    __shared__ alignas(16) uint2 s_gathered[kSelect && kLanes == 32 ? kWarps : 1][32];
+    __shared__ alignas(16) uint2 s_gathered[kChoose >= kRank ? kWarps : 1][32];
     __shared__ float s_z[kWarps], s_part[kWarps], s_parts[kCluster];
     __shared__ int s_rows[kWarps], s_routes;
     int* const hist = reinterpret_cast<int*>(smem + kSumRows * Row::kFloats);
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
     float2* const chosen = reinterpret_cast<float2*>(hist + ((g.E + 1) & ~1)) + static_cast<size_t>(group) * g.K;
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0 && !g.one_launch) *g.ticket = 0;
-    const int set = kLanes == 32 && kChoose == kFew ? set_of<V>(g.E, g.K) : 0;
+    const int set = kChoose == kRank ? set_of<V>(g.E, g.K) : 0;
     const long long first = static_cast<long long>(blockIdx.x) * g.rows_per_block;
     int pos = static_cast<int>(min(first, static_cast<long long>(g.T)));
     const int hi = static_cast<int>(min(first + g.rows_per_block, static_cast<long long>(g.T)));
@@ -304,9 +304,9 @@ __global__ void __launch_bounds__(kRowThreads, row_blocks_per_sm(kLanes * V)) ba
             float max_known;
             if constexpr (kSelect) {
                 const unsigned o = static_cast<unsigned>(t) * static_cast<unsigned>(g.K);        // a call has fewer than 2^31 routes
-                if constexpr (kLanes != 32) {
+                if constexpr (kChoose == kRounds) {
                     rounds<kLanes, V>(v, g.E, g.K, chosen);
-                } else if constexpr (kChoose == kFew) {
+                } else if constexpr (kChoose == kRank) {
                     select_by_rank<V>(v, g.E, g.K, set, s_gathered[warp], chosen);
                 } else {
                     select_many<V>(v, g.E, g.K, s_gathered[warp], chosen);
@@ -609,8 +609,15 @@ int launch_rows(const BalanceParams& p, cudaStream_t s) {
 template <typename T, int kLanes, int V, bool kSigmoid>
 int launch_choice(const BalanceParams& p, cudaStream_t s) {
     if (p.top_in != nullptr) return launch_rows<T, kLanes, V, kSigmoid, kNone>(p, s);
-    if constexpr (kLanes == 32) if (p.K > 16) return launch_rows<T, kLanes, V, kSigmoid, kMany>(p, s);
-    return launch_rows<T, kLanes, V, kSigmoid, kFew>(p, s);
+    // Rows that share a warp cannot choose by rank.  Sorted rounds cost every route the same, ranks little for one more: 131072 x
+    // 128, forward, rounds and rank: K = 1 39 and 51 us, 4 48 and 55, 8 59 and 60, 16 80 and 71.
+    if constexpr (kLanes < 32) {
+        return launch_rows<T, kLanes, V, kSigmoid, kRounds>(p, s);
+    } else {
+        if (p.K > 16) return launch_rows<T, kLanes, V, kSigmoid, kMany>(p, s);
+        if constexpr (V == 4) if (p.K <= 8) return launch_rows<T, kLanes, V, kSigmoid, kRounds>(p, s);
+        return launch_rows<T, kLanes, V, kSigmoid, kRank>(p, s);
+    }
 }
 template <typename T, int kLanes, int V>
 int launch_rows_as(const BalanceParams& p, cudaStream_t s) {
