@@ -611,6 +611,7 @@ int launch_choice(const BalanceParams& p, cudaStream_t s) {
     if (p.top_in != nullptr) return launch_rows<T, kLanes, V, kSigmoid, kNone>(p, s);
     // Rows that share a warp cannot choose by rank.  Sorted rounds cost every route the same, ranks little for one more: 131072 x
     // 128, forward, rounds and rank: K = 1 39 and 51 us, 4 48 and 55, 8 59 and 60, 16 80 and 71.
+    // Rows of 256 lose from four routes on, with three kept values a lane: K = 1 57 and 64, 2 62 and 64, 4 73 and 67, 8 93 and 73.
     if constexpr (kLanes < 32) {
         return launch_rows<T, kLanes, V, kSigmoid, kRounds>(p, s);
     } else {
