@@ -543,8 +543,9 @@ __global__ void __launch_bounds__(kBwdThreads, bwd_blocks_per_sm(V, kSigmoid)) b
             dot = group_sum<kLanes>(dot);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                dw[i] = w[i] == 0.0f ? 0.0f : w[i] * (dw[i] - dot);
-                if (kSigmoid && expert[i] >= 0) dw[i] *= sigmoid_rest(to_float(row[expert[i]]));
+                float slope = w[i] * (dw[i] - dot);
+                if (kSigmoid && expert[i] >= 0) slope *= sigmoid_rest(to_float(row[expert[i]]));
+                dw[i] = w[i] == 0.0f ? 0.0f : slope;       // last: a route of weight 0 takes nothing, its logit may be NaN
                 if (expert[i] >= 0) {
                     expert[i] = Row::at(expert[i]);                // from here on its place in the shared row
                     add[expert[i]] = __int_as_float(l + i * kLanes);
