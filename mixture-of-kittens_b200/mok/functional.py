@@ -414,6 +414,11 @@ class _RouteBalanced(torch.autograd.Function):
     backward = staticmethod(torch.autograd.function.once_differentiable(ops._topk_balance_backward))
 
 
+def _one_loss_a_group(group: dist.ProcessGroup | None, sequence_offsets: torch.Tensor | None) -> None:
+    if group is not None and sequence_offsets is not None:
+        raise ValueError("counts of a group belong to one loss over the whole batch: pass no sequence_offsets")
+
+
 def balance_loss(logits: torch.Tensor, top_experts: torch.Tensor, *, token_mask: torch.Tensor | None = None,
                  sequence_offsets: torch.Tensor | None = None, score: str = "softmax",
                  group: dist.ProcessGroup | None = None) -> MoKBalance:
@@ -422,10 +427,9 @@ def balance_loss(logits: torch.Tensor, top_experts: torch.Tensor, *, token_mask:
     int32; averaged over ranks with as many tokens that count each, it is the loss of the global batch); `counts` stays
     local."""
     sigmoid = _sigmoid_score(score)
+    _one_loss_a_group(group, sequence_offsets)
     load = None
     if group is not None:
-        if sequence_offsets is not None:
-            raise ValueError("counts of a group belong to one loss over the whole batch: pass no sequence_offsets")
         load = ops.expert_counts(top_experts, logits.shape[-1], token_mask)
         dist.all_reduce(load, group=group)
     losses, counts, _ = _Balance.apply(logits, top_experts, token_mask, sequence_offsets, load, sigmoid)
@@ -438,6 +442,7 @@ def route_balanced(logits: torch.Tensor, topk: int, *, token_mask: torch.Tensor 
     """route() with the losses of `balance_loss` from the same pass over the logits: (top_experts int64 [T, K], router_weights
     f32 [T, K], MoKBalance).  `score` "sigmoid" weighs the chosen experts by their sigmoids over the sum of them."""
     sigmoid = _sigmoid_score(score)
+    _one_loss_a_group(group, sequence_offsets)
     experts, weights, losses, counts, _ = _RouteBalanced.apply(logits, topk, token_mask, sequence_offsets, sigmoid)
     if group is not None:              # the loss needs the other ranks' counts, which follow from the choice
         return experts, weights, balance_loss(logits, experts, token_mask=token_mask, sequence_offsets=sequence_offsets,
