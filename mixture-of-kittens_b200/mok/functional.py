@@ -457,6 +457,9 @@ def route_balanced_and_schedule(workspace: MoKWorkspace, config: MoKConfig, logi
     """route_balanced() + build_schedule(): (schedule, top_experts, router_weights, MoKBalance)."""
     if not isinstance(workspace, MoKWorkspace):
         raise TypeError("workspace must be a MoKWorkspace")
+    if not isinstance(config, MoKConfig):
+        raise TypeError("config must be a MoKConfig")
+    _validate_config(config, workspace)
     if type(num_local_experts) is not int or num_local_experts <= 0:
         raise ValueError("num_local_experts must be a positive integer")
     if logits.ndim != 2 or logits.shape[0] != workspace.num_local_tokens:

@@ -108,3 +108,23 @@ def test_a_group_with_sequences_is_refused_before_any_work(monkeypatch):
         F.route_balanced(logits, 2, sequence_offsets=offsets, group=object())
     with pytest.raises(ValueError, match="sequence_offsets"):
         F.balance_loss(logits, torch.zeros(8, 2, dtype=torch.int64), sequence_offsets=offsets, group=object())
+
+
+def test_a_wrong_configuration_is_refused_before_any_work(monkeypatch):
+    """As route_and_schedule does: nothing is routed and no count summed for a schedule that cannot be built."""
+    import dataclasses
+    from types import SimpleNamespace
+    from mok import functional as F, ops
+    stop = lambda *a, **k: pytest.fail("work before the refusal")                        # noqa: E731
+    for name in ("router_topk_balance", "router_topk_gather", "router_balance", "expert_counts"):
+        monkeypatch.setattr(ops, name, stop)
+    monkeypatch.setattr(F, "_device_properties", lambda device: SimpleNamespace(multi_processor_count=148, shared_memory_per_block_optin=232448))
+    fields = {f.name: None for f in dataclasses.fields(F.MoKWorkspace)}
+    ws = F.MoKWorkspace(**{**fields, "device": torch.device("cpu"), "num_local_tokens": 512, "topk": 2, "ep_size": 1, "ep_rank": 0})
+    logits = torch.zeros(512, 8)
+    for route in (F.route_and_schedule, F.route_balanced_and_schedule):
+        for config in (F.MoKConfig(fwd_num_comm_sms=3), F.MoKConfig(minibatch_size=100)):
+            with pytest.raises(ValueError):
+                route(ws, config, logits, num_local_experts=8)
+        with pytest.raises(TypeError):
+            route(ws, None, logits, num_local_experts=8)
