@@ -485,8 +485,9 @@ def dropout_add(x: torch.Tensor, residual: torch.Tensor | None = None, *, p: flo
                 seed: torch.Tensor | None = None) -> torch.Tensor:
     """residual + dropout(x) (x alone without a residual), the layer's exit in a transformer block; see `ops.dropout_add`.
     `seed` is an int64 tensor [1] on the device; without one it is drawn from torch's generator of that device, so
-    torch.manual_seed, activation checkpoints and captured graphs treat it like any other random number.  Not training, or
-    with p = 0, nothing is dropped and no seed drawn."""
+    torch.manual_seed, activation checkpoints and captured graphs treat it like any other random number.  Layouts other than
+    contiguous are copied first; an element's number follows its place in x's shape.  Not training, or with p = 0, nothing is
+    dropped, no seed drawn and the sum is torch's own, of any type and device."""
     if type(p) not in (float, int) or not 0 <= p <= 1:
         raise ValueError("p must be a number in [0, 1]")
     if not training or p == 0:
@@ -497,7 +498,7 @@ def dropout_add(x: torch.Tensor, residual: torch.Tensor | None = None, *, p: flo
         return x + residual
     if seed is None:
         seed = torch.randint(0, 2 ** 63 - 1, (1,), dtype=torch.int64, device=x.device)
-    return _DropoutAdd.apply(x, residual, seed, p)
+    return _DropoutAdd.apply(x.contiguous(), None if residual is None else residual.contiguous(), seed, p)
 
 
 def validate_inputs(config: MoKConfig, workspace: MoKWorkspace, schedule: MoKSchedule, x: torch.Tensor,
