@@ -29,8 +29,17 @@ constexpr int kWarps = 16;
 constexpr int kRowThreads = kWarps * 32;
 constexpr int kBwdThreads = 256;
 // Blocks of the backward pass that an SM has to be able to hold, which bounds their registers; the grid is twice as many.
-// One B200, us: 131072 x 256 f32 with five 53, four 58, six 55; 65536 x 500 bf16 with four 56, two 70, sigmoid scores 30000 x 500
-// with three 36, four (spills) 44; 30000 x 1024 f32 with two 63, three (spills) 88 to 92.
+// One B200, us, losses alone and with the router weights' gradient:
+//   131072 x 256 f32                     three 52 and 68   four 47 and 58   five 45 and 54   six 47 and 54
+//   the same with sigmoid scores                83              76               77               83  (with the weights)
+//   65536 x 500 bf16, 61 sequences       two 49            three 42         four 39          five 51  (losses alone)
+//   30000 x 500 f32, sigmoid scores      two 34 and 41     three 36 and 43  four 45 and 51
+//   the same in bf16                         34 and 44           34 and 42       40 and 48
+//   30000 x 1024 f32                     one 50 and 58     two 43 and 46    three 59 and 65
+//   the same with sigmoid scores             69 and 83         71 and 81         148 and 158
+//   the same in bf16                         80 and 101        71 and 81         125 and 137
+// One block fewer spills nothing.  Those chosen store 12 spilled bytes at 512 experts, with sigmoid scores up to 52 at 256 and fewer, 136
+// at 512, 436 (f32) and 476 at 1024; one block more 172 to 412, with sigmoid scores 240 to 948, above 256 experts.
 constexpr int bwd_blocks_per_sm(int V, bool sigmoid) { return V <= 8 ? 5 : V == 16 ? 4 - sigmoid : 2; }
 constexpr int kSumRows = kWarps / 2;           // rows of E sums in shared memory that a block's warps share, two to a row
 // Blocks of the forward pass, all resident at once on 148 SMs: two an SM up to 512 experts, one above (their rows take twice

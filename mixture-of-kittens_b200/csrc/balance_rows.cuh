@@ -230,8 +230,10 @@ __device__ __forceinline__ void select_many(float (&v)[V], int E, int K, uint2* 
 }
 
 // Bound by instructions and, without the choice, by the latency of its loads.  Reads T E logits once, writes K routes a row and (p,
-// routes) per slot.  One B200 with the join, us (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 74 (21), finished routes
-// 36; 65536 x 500 bf16, K = 6, 61 sequences: 69 (10) and 32; 16384 x 128: 15 (1.3) and 10.  A row of 256 takes 470 instructions
+// routes) per slot.  One B200 with the join, us, inputs not in the cache (floor: bytes at 6456 GB/s): 131072 x 256 f32, K = 8: 71 (23),
+// finished routes 35; 65536 x 500 bf16, K = 6, 61 sequences: 69 (11) and 35; 16384 x 128: 15 (1.5) and 12; 30000 x 1024 f32, K = 8: 49 (19) and
+// 30.  Sigmoid scores 131072 x 256: 92, 65536 x 500 bf16 without sequences: 85 against 62.  With the choice of 1024 and 512 experts and of
+// more than 16 routes the registers do not suffice: 4 to 140 bytes are spilled.  A row of 256 takes 470 instructions
 // with the choice, 130 without; in rounds of one maximum each the choice alone took 540.  Loading the next row ahead: 53 -> 44
 // without the choice at 256 experts; above, the registers it takes cost more (36 -> 46 at 500).  Finished routes are counted for a
 // run's rows at once; with their row, each row waited for its ids (44 -> 36).  Rows staged in shared memory two to four ahead by
@@ -612,7 +614,8 @@ int launch_choice(const BalanceParams& p, cudaStream_t s) {
     if (p.top_in != nullptr) return launch_rows<T, kLanes, V, kSigmoid, kNone>(p, s);
     // Rows that share a warp cannot choose by rank.  Sorted rounds cost every route the same, ranks little for one more: 131072 x
     // 128, forward, rounds and rank: K = 1 39 and 51 us, 4 48 and 55, 8 59 and 60, 16 80 and 71.
-    // Rows of 256 lose from four routes on, with three kept values a lane: K = 1 57 and 64, 2 62 and 64, 4 73 and 67, 8 93 and 73.
+    // Rows of 256 lose from four routes on, with three kept values a lane: K = 1 57 and 64, 2 62 and 64, 4 73 and 67, 8 93 and 73.  What
+    // that wins at one and two routes was not thought worth four kernels more.
     if constexpr (kLanes < 32) {
         return launch_rows<T, kLanes, V, kSigmoid, kRounds>(p, s);
     } else {

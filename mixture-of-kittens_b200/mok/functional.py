@@ -403,7 +403,7 @@ class _Balance(torch.autograd.Function):
 
 
 class _RouteBalanced(torch.autograd.Function):
-    """router_topk_balance on the autograd tape: one launch gives the gradient of the weights and of both losses."""
+    """router_topk_balance on the autograd tape: one launch gives the gradient of the weights and, without a group, of both losses."""
 
     @staticmethod
     def forward(ctx, logits, topk, token_mask, sequence_offsets, sigmoid):
@@ -440,7 +440,8 @@ def route_balanced(logits: torch.Tensor, topk: int, *, token_mask: torch.Tensor 
                    sequence_offsets: torch.Tensor | None = None, score: str = "softmax",
                    group: dist.ProcessGroup | None = None) -> tuple[torch.Tensor, torch.Tensor, MoKBalance]:
     """route() with the losses of `balance_loss` from the same pass over the logits: (top_experts int64 [T, K], router_weights
-    f32 [T, K], MoKBalance).  `score` "sigmoid" weighs the chosen experts by their sigmoids over the sum of them."""
+    f32 [T, K], MoKBalance).  `score` "sigmoid" weighs the chosen experts by their sigmoids over the sum of them.  With `group` the
+    losses wait for the other ranks' counts and take a second pass over the logits, and their gradient a launch of its own."""
     sigmoid = _sigmoid_score(score)
     _one_loss_a_group(group, sequence_offsets)
     experts, weights, losses, counts, _ = _RouteBalanced.apply(logits, topk, token_mask, sequence_offsets, sigmoid)

@@ -71,7 +71,8 @@ class MoKLayer(torch.nn.Module):
     ``forward(x)`` routes with the layer's own router; ``forward(x, top_experts, router_weights)`` takes finished
     routes (int64 [T, K], f32 [T, K]) as ``functional.build_schedule`` / ``functional.forward`` do.
 
-    ``score`` "sigmoid" weighs the chosen experts by sigmoids instead of the softmax.  ``dropout`` is applied to the layer's
+    ``score`` "sigmoid" weighs the chosen experts by sigmoids instead of the softmax (by the router that also computes the
+    losses, asked for or not).  ``dropout`` is applied to the layer's
     output while training; ``residual`` is added behind it in the same pass.  With ``return_balance`` the call returns
     (output, functional.MoKBalance) for the tokens that ``token_mask`` and ``sequence_offsets`` leave (see
     ``functional.balance_loss``); ``balance_group`` makes the loss that of the global batch of its ranks.
